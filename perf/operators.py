@@ -17,10 +17,10 @@ With ``own`` false, ``run`` computes them with elementary torch operations in
 32 bits (64 for the random scores); with ``own`` true it calls the
 ``src.kernels`` entry points.
 
-4-bit storage: a row is cut into tiles of 128 columns (the last one padded),
-a tile is 16 int32 words, word 4 t + j of which holds columns 32 j + 8 t ..
-+ 7: column + 0, 2, 4, 6 in bits 0, 4, 8, 12 and column + 1, 3, 5, 7 in bits
-16, 20, 24, 28.
+4-bit storage: blocks of 16 rows by 128 columns (both padded) follow each
+other along a row of blocks: codes (ceil(N / 16), ceil(K / 128), 16, 16) int32.
+Word 4 t + j of a block's row holds its columns 32 j + 8 t .. + 7: column + 0,
+2, 4, 6 in bits 0, 4, 8, 12 and column + 1, 3, 5, 7 in bits 16, 20, 24, 28.
 """
 
 import os
@@ -129,8 +129,8 @@ def prepare(case, seed):
 
 def _prepare_w4(c, g):
     N, K, G = c["N"], c["K"], c["G"]
-    tiles, groups = -(-K // 128), -(-K // G)
-    codes = torch.zeros(N, tiles * 16, dtype=torch.int32, device="cuda")
+    groups = -(-K // G)
+    codes = torch.zeros(-(-N // 16), -(-K // 128), 16, 16, dtype=torch.int32, device="cuda")
     for shift in range(0, 32, 4):  # bell-shaped codes, as rounded weights have them
         q = torch.randn(codes.shape, generator=g, device="cuda").mul_(2.6).add_(8.0).round_().clamp_(0, 15)
         codes |= q.to(torch.int32) << shift
@@ -199,10 +199,10 @@ def run(state):
 
 def _plain_w4(x, codes, scales, zeros, group):
     M, K = x.shape
-    N = codes.shape[0]
+    N = scales.shape[0]
     shifts = torch.tensor(NIBBLE_SHIFTS, dtype=torch.int32, device=x.device)
-    words = codes.view(N, -1, 4, 4).transpose(2, 3).reshape(N, -1, 1)
-    w = ((words >> shifts) & 15).reshape(N, -1)[:, :K].float()
+    words = codes.unflatten(3, (4, 4)).permute(0, 2, 1, 4, 3)  # [rows / 16][row][columns / 128][j][t]
+    w = ((words.unsqueeze(-1) >> shifts) & 15).flatten(0, 1).flatten(1)[:N, :K].float()
     at = torch.arange(K, device=x.device) // group
     w = w - (8.0 if zeros is None else zeros.float()[:, at])
     w = w * scales.float()[:, at]
@@ -312,16 +312,17 @@ def _exact_w4(c, s):
     N, K, G = c["N"], c["K"], c["G"]
     x = s["x"].double()
     y = torch.empty(c["M"], N, dtype=torch.float64, device="cuda")
-    # place[k]: (word, bit) of column k
+    # (word, bit) of column k in a row of 16 words a block
     k = np.arange(K)
     tile, inner = k // 128, k % 128
     word = tile * 16 + 4 * ((inner % 32) // 8) + inner // 32
     bit = 4 * ((inner % 8) // 2) + 16 * (inner % 2)
     word_t, bit_t = torch.from_numpy(word).cuda(), torch.from_numpy(bit).cuda()
+    words = s["codes"].transpose(1, 2).reshape(-1, (K + 127) // 128 * 16)
     rows = max(1, (1 << 24) // K)
     for n0 in range(0, N, rows):
         part = slice(n0, min(N, n0 + rows))
-        code = (s["codes"][part].long()[:, word_t] >> bit_t) % 16
+        code = (words[part].long()[:, word_t] >> bit_t) % 16
         w = code.double()
         for g0 in range(0, K, G):
             cols, grp = slice(g0, min(K, g0 + G)), g0 // G
