@@ -1,0 +1,442 @@
+// Products with 4-bit weights: y[m, n] = sum_k x[m, k] (q[n, k] - z[n, G]) s[n, G].
+//
+// For the batches a token step has, the call is a stream of the codes (half
+// a byte a weight); everything else has to fit under it.
+//
+//   * q - z is an integer of at most 5 bits, exact in bf16, and 128 + q is
+//     the bf16 whose mantissa ends in q: a pair of codes becomes a bf16 pair
+//     with one mask-and-or and one packed subtraction of 128 + z.
+//   * mma.sync.m16n8k16 (bf16 in, fp32 sums) takes the 16 weight rows as its
+//     M and 8 batch rows as its N, so one batch row costs no more than eight.
+//     Products of a bf16 x are exact; an fp32 x is cut into three bf16 terms
+//     of 8 significant bits each (24 together, all of x) and takes three MMAs.
+//   * The scale is applied to the fp32 sum of a group, not to the weight:
+//     nothing is rounded below fp32 before the output.
+//   * The order of k is free.  A block of 16 rows by 128 columns is 1 KB in
+//     which lane (g, t) of a warp reads 16 bytes of row g and of row g + 8
+//     (words 4 t + j, j = 0..3): two contiguous 512-byte loads.  Word j of a
+//     row's four lanes is the columns 32 j + 8 t .. + 7, a 32-column run: two
+//     MMAs, and the finest group.  The batch operand of both is the 8
+//     consecutive elements of x at the same columns.
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "m3_kernels.cuh"
+#include "m3_lm.cuh"
+
+namespace m3 {
+
+namespace {
+
+struct W4Params {
+  int M, N, K, tiles, blocks;  // tiles: 128-column tiles, blocks: 16-row blocks
+  int wk, wn;                   // warps along K, row blocks at a time, of a CTA
+  int mtiles;                   // batch tiles; a CTA works for one
+  const void *x;
+  int64_t ldx;
+  int x_vec;  // every row of x starts on 16 bytes
+  const uint4 *codes;
+  const void *scales;
+  int64_t s_ld;
+  int s_bf16, groups;
+  const uint8_t *zeros;
+  int64_t z_ld;
+  void *y;
+  int64_t ldy;
+  int y_bf16;
+};
+
+__device__ __forceinline__ void w4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// pair i of a word as bf16 (q - z), with zz = (128 + z, 128 + z)
+__device__ __forceinline__ uint32_t w4_pair(uint32_t w, int i, uint32_t zz) {
+  uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&v), *reinterpret_cast<__nv_bfloat162 *>(&zz));
+  return *reinterpret_cast<uint32_t *>(&d);
+}
+
+// 16 bytes of codes, read once: past L1.  Volatile, so that it stays behind
+// the wait for the preceding kernel.
+__device__ __forceinline__ uint4 w4_codes(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// 8 consecutive elements of a batch row as bf16 terms: one for bf16 x, three
+// for fp32 x (head, middle, rest; each the truncation of what is left, so
+// that head + middle + rest is x).  An infinite x is its head alone.
+template <typename XT>
+struct W4X;
+
+template <>
+struct W4X<__nv_bfloat16> {
+  static constexpr int kTerms = 1;
+  uint4 t[1];
+  __device__ __forceinline__ void load(const void *x, int64_t row, int k, int K, bool vec) {
+    const __nv_bfloat16 *p = static_cast<const __nv_bfloat16 *>(x) + row + k;
+    if (vec && k + 8 <= K) {
+      t[0] = *reinterpret_cast<const uint4 *>(p);
+      return;
+    }
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (uint32_t)__bfloat16_as_ushort(p[i]) : 0u;
+    t[0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+  __device__ __forceinline__ void zero() { t[0] = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void terms(uint4 (&o)[1]) const { o[0] = t[0]; }
+};
+
+template <>
+struct W4X<float> {
+  static constexpr int kTerms = 3;
+  float v[8];
+  __device__ __forceinline__ void load(const void *x, int64_t row, int k, int K, bool vec) {
+    const float *p = static_cast<const float *>(x) + row + k;
+    if (vec && k + 8 <= K) {
+      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+  __device__ __forceinline__ void terms(uint4 (&o)[3]) const {
+    uint32_t h[8], m[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[i] = __float_as_uint(v[i]);
+      const float r = isinf(v[i]) ? 0.f : v[i] - __uint_as_float(h[i] & 0xffff0000u);
+      m[i] = __float_as_uint(r);
+      l[i] = __float_as_uint(r - __uint_as_float(m[i] & 0xffff0000u));
+    }
+    auto pack = [](const uint32_t (&b)[8]) {
+      return make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632),
+                        __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
+    };
+    o[0] = pack(h), o[1] = pack(m), o[2] = pack(l);
+  }
+};
+
+// One block's codes and scales of a warp, in registers.
+template <int GPT>
+struct W4Stage {
+  uint4 c[2];
+  float s[2][GPT];
+  uint32_t z[2][GPT];
+};
+
+// Block (rb, kt) of the weight: rows 16 rb + g and + 8.
+template <int GPT>
+__device__ __forceinline__ void w4_load(W4Stage<GPT> &st, const W4Params &p, int rb, int kt, int lane) {
+  const uint4 *c = p.codes + ((int64_t)rb * p.tiles + kt) * 64 + lane;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    st.c[h] = w4_codes(c + h * 32);
+    const int64_t n = min(rb * 16 + h * 8 + (lane >> 2), p.N - 1);  // rows past the last reach no output
+#pragma unroll
+    for (int j = 0; j < GPT; ++j) {
+      const int gi = min(kt * GPT + j, p.groups - 1);  // a group wholly past K has a sum of 0
+      st.s[h][j] = p.s_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.scales)[n * p.s_ld + gi])
+                            : static_cast<const float *>(p.scales)[n * p.s_ld + gi];
+      const uint32_t z = p.zeros ? (uint32_t)p.zeros[n * p.z_ld + gi] : 8u;
+      st.z[h][j] = 0x43004300u + z + (z << 16);
+    }
+  }
+}
+
+// tot += the block's products with MT 8-row batch tiles; get(o, j, b) gives
+// the terms of x for run j of the tile and batch tile b.
+template <int MT, int GPT, int TERMS, typename Get>
+__device__ __forceinline__ void w4_block(float (&tot)[MT][4], const W4Stage<GPT> &st, Get get) {
+  constexpr int PER = 4 / GPT;  // 32-column runs of a group
+  float d[MT][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int gj = j / PER;
+    if (j % PER == 0) {
+#pragma unroll
+      for (int b = 0; b < MT; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[b][e] = 0.f;
+    }
+    uint32_t w[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t word = j == 0 ? st.c[h].x : j == 1 ? st.c[h].y : j == 2 ? st.c[h].z : st.c[h].w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[h][i] = w4_pair(word, i, st.z[h][gj]);
+    }
+#pragma unroll
+    for (int b = 0; b < MT; ++b) {
+      uint4 o[TERMS];
+      get(o, j, b);
+#pragma unroll
+      for (int q = TERMS - 1; q >= 0; --q) {  // small terms first
+        w4_mma(d[b], w[0][0], w[1][0], w[0][1], w[1][1], o[q].x, o[q].y);
+        w4_mma(d[b], w[0][2], w[1][2], w[0][3], w[1][3], o[q].z, o[q].w);
+      }
+    }
+    if (j % PER == PER - 1) {
+#pragma unroll
+      for (int b = 0; b < MT; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tot[b][e] = fmaf(d[b][e], st.s[e >> 1][gj], tot[b][e]);
+    }
+  }
+}
+
+__device__ __forceinline__ void w4_store(const W4Params &p, int m, int n, float s) {
+  if (p.y_bf16)
+    static_cast<__nv_bfloat16 *>(p.y)[(int64_t)m * p.ldy + n] = __float2bfloat16_rn(s);
+  else
+    static_cast<float *>(p.y)[(int64_t)m * p.ldy + n] = s;
+}
+
+constexpr int kW4Warps = 16;
+constexpr int kW4Depth = 3;                   // blocks a warp has in flight
+constexpr int kW4SmemBudget = 200 * 1024;     // x and the partial sums
+
+// Partial sums of a warp: 16 rows by MT * 8 batch rows, padded against bank conflicts
+constexpr int kW4RowLd = 17;
+template <int MT>
+constexpr int w4_red_floats() { return MT * 8 * kW4RowLd; }
+
+// x as the MMAs take it: [tile][run j][batch tile][term][lane] pieces of 16 bytes
+template <int MT, int TERMS>
+int64_t w4_stream_smem(int tiles, int wk, int wn) {
+  return (int64_t)tiles * 4 * MT * TERMS * 512 + (int64_t)2 * wk * wn * w4_red_floats<MT>() * 4;
+}
+
+// The decode batches' kernel: persistent CTAs that hold all of x in shared
+// memory, in fragment order, and stream blocks of codes through registers,
+// kW4Depth ahead.  A CTA's p.wk x p.wn warps are p.wn groups; a group takes
+// row blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of one, and
+// their sums are added in warp order through shared memory (two buffers and
+// one barrier of the group per row block).
+template <typename XT, int MT, int GPT>
+__global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Params p) {
+  using X = W4X<XT>;
+  constexpr int TERMS = X::kTerms, RED = w4_red_floats<MT>();
+  extern __shared__ __align__(16) uint4 w4_smem[];
+  const int pieces = p.tiles * 4 * MT * 32;
+  float *red = reinterpret_cast<float *>(w4_smem + (int64_t)pieces * TERMS);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wk = warp % p.wk, wn = warp / p.wk;
+  const int m0 = (int)(blockIdx.x % p.mtiles) * MT * 8, rows = min(p.M - m0, MT * 8);
+  const int rb0 = (int)(blockIdx.x / p.mtiles) * p.wn + wn, rstep = (int)(gridDim.x / p.mtiles) * p.wn;
+  const int spt = (p.tiles + p.wk - 1) / p.wk;  // steps of a row block
+  const int rounds = rb0 < p.blocks ? (p.blocks - rb0 + rstep - 1) / rstep : 0;
+  const int total = rounds * spt;
+
+  // the first blocks into L2 while the preceding kernel runs
+  if (total > 0 && wk == 0 && lane == 0) {
+    const uint32_t bytes = (uint32_t)min(p.tiles, kW4Depth * p.wk) * 1024u;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.codes + (int64_t)rb0 * p.tiles * 64),
+                 "r"(bytes)
+                 : "memory");
+  }
+  pdl_wait();  // x is the preceding kernel's output, and the weight may be too
+  pdl_trigger();
+
+  int lrb = rb0, lk = wk;  // the next block to load
+  auto load = [&](W4Stage<GPT> &st) {
+    if (lrb < p.blocks && lk < p.tiles) w4_load(st, p, lrb, lk, lane);
+    lk += p.wk;
+    if (lk >= spt * p.wk) lk = wk, lrb += rstep;
+  };
+  W4Stage<GPT> st[kW4Depth];
+#pragma unroll
+  for (int u = 0; u < kW4Depth; ++u) load(st[u]);
+
+  for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+    const int l = i & 31, b = (i >> 5) % MT, kj = (i >> 5) / MT;
+    const int m = b * 8 + (l >> 2);
+    X xv;
+    if (m < rows)
+      xv.load(p.x, (int64_t)(m0 + m) * p.ldx, kj * 32 + 8 * (l & 3), p.K, p.x_vec);
+    else
+      xv.zero();
+    uint4 o[TERMS];
+    xv.terms(o);
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q) w4_smem[((i >> 5) * TERMS + q) * 32 + l] = o[q];
+  }
+  __syncthreads();
+
+  float tot[MT][4];
+  int step = 0, kt = wk, rb = rb0, parity = 0;
+  for (int it = 0; it < total; it += kW4Depth) {
+#pragma unroll
+    for (int u = 0; u < kW4Depth; ++u) {
+      if (it + u < total) {
+        if (step == 0) {
+#pragma unroll
+          for (int b = 0; b < MT; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
+        }
+        if (kt < p.tiles) {
+          const uint4 *xs = w4_smem + (int64_t)kt * 4 * MT * TERMS * 32 + lane;
+          w4_block<MT, GPT, TERMS>(tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
+#pragma unroll
+            for (int q = 0; q < TERMS; ++q) o[q] = xs[((j * MT + b) * TERMS + q) * 32];
+          });
+        }
+        load(st[u]);
+        kt += p.wk;
+        if (++step == spt) {
+          // element e of a tile: weight row g + 8 (e / 2), batch row 2 t + e % 2
+          float *group = red + (parity * p.wn + wn) * p.wk * RED;
+          float *mine = group + wk * RED;
+#pragma unroll
+          for (int b = 0; b < MT; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mine[(b * 8 + 2 * (lane & 3) + (e & 1)) * kW4RowLd + (e >> 1) * 8 + (lane >> 2)] = tot[b][e];
+          asm volatile("bar.sync %0, %1;" ::"r"(wn + 1 <= 15 ? wn + 1 : 0), "r"(p.wk * 32) : "memory");
+          for (int i = wk * 32 + lane; i < rows * 16; i += p.wk * 32) {
+            const int r = i & 15, m = i >> 4, n = rb * 16 + r;
+            float s = group[m * kW4RowLd + r];
+            for (int k = 1; k < p.wk; ++k) s += group[k * RED + m * kW4RowLd + r];
+            if (n < p.N) w4_store(p, m0 + m, n, s);
+          }
+          parity ^= 1, step = 0, kt = wk, rb += rstep;
+        }
+      }
+    }
+  }
+}
+
+// Any batch and any K: the same blocks, x read where it is.  A CTA is 8 warps,
+// 2 along K by 4 row blocks that share x through L1.
+template <typename XT, int MT, int GPT>
+__global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mtiles) {
+  using X = W4X<XT>;
+  constexpr int WK = 2, WN = 4, COLS = MT * 8;
+  __shared__ float red[WN][WK][w4_red_floats<MT>()];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int wk = warp % WK, wn = warp / WK;
+  const int m0 = (int)(blockIdx.x % mtiles) * COLS;
+  const int rb = min((int)(blockIdx.x / mtiles) * WN + wn, p.blocks - 1);  // past the last: computed, not stored
+  float tot[MT][4];
+#pragma unroll
+  for (int b = 0; b < MT; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
+  pdl_wait();
+  pdl_trigger();
+  W4Stage<GPT> cur, nxt;
+  if (wk < p.tiles) w4_load(cur, p, rb, wk, lane);
+  for (int kt = wk; kt < p.tiles; kt += WK) {
+    if (kt + WK < p.tiles) w4_load(nxt, p, rb, kt + WK, lane);
+    w4_block<MT, GPT, X::kTerms>(tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
+      const int m = m0 + b * 8 + g;
+      X xv;
+      if (m < p.M)
+        xv.load(p.x, (int64_t)m * p.ldx, kt * M3_W4_TILE + 32 * j + 8 * t, p.K, p.x_vec);
+      else
+        xv.zero();
+      xv.terms(o);
+    });
+    cur = nxt;
+  }
+#pragma unroll
+  for (int b = 0; b < MT; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[wn][wk][(b * 8 + 2 * t + (e & 1)) * kW4RowLd + (e >> 1) * 8 + g] = tot[b][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < COLS * WN * 16; i += 256) {
+    const int r = i & 15, w = (i >> 4) % WN, c = i / (WN * 16);
+    const int m = m0 + c, n = ((int)(blockIdx.x / mtiles) * WN + w) * 16 + r;
+    if (m < p.M && n < p.N) w4_store(p, m, n, red[w][0][c * kW4RowLd + r] + red[w][1][c * kW4RowLd + r]);
+  }
+}
+
+template <typename XT, int MT, int GPT>
+cudaError_t launch_w4_direct(const W4Params &p, cudaStream_t stream) {
+  const int mtiles = (p.M + MT * 8 - 1) / (MT * 8);
+  const int64_t grid = (int64_t)((p.blocks + 3) / 4) * mtiles;
+  if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_pdl(w4_direct_kernel<XT, MT, GPT>, dim3((unsigned)grid), dim3(256), 0, stream, p, mtiles);
+}
+
+// Warps along K: the split with the fewest steps of the busiest warp (fewest
+// warps a row block on ties: less to add up), then as many row blocks per CTA
+// as keep every SM busy.
+template <typename XT, int MT, int GPT>
+cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
+  constexpr int TERMS = W4X<XT>::kTerms;
+  p.mtiles = (p.M + MT * 8 - 1) / (MT * 8);
+  const int sms = max(1, sm_count_current() / p.mtiles);  // of a batch tile
+  int64_t best = INT64_MAX;
+  for (int wk = 1; wk <= kW4Warps; wk *= 2) {
+    const int64_t streams = (int64_t)sms * (kW4Warps / wk);
+    const int64_t steps = (p.blocks + streams - 1) / streams * ((p.tiles + wk - 1) / wk);
+    if (steps < best) best = steps, p.wk = wk;
+  }
+  p.wn = min(kW4Warps / p.wk, (p.blocks + sms - 1) / sms);
+  const int64_t smem = w4_stream_smem<MT, TERMS>(p.tiles, p.wk, p.wn);
+  *taken = smem <= kW4SmemBudget;
+  if (!*taken) return cudaSuccess;
+  auto kern = w4_stream_kernel<XT, MT, GPT>;
+  static LaunchCache cache;
+  if (cudaError_t e = ensure_smem_optin(cache, kern, kW4SmemBudget); e != cudaSuccess) return e;
+  const int64_t grid = (int64_t)min(sms, (p.blocks + p.wn - 1) / p.wn) * p.mtiles;
+  if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_pdl(kern, dim3((unsigned)grid), dim3(p.wk * p.wn * 32), (size_t)smem, stream, p);
+}
+
+template <typename XT, int GPT>
+cudaError_t launch_w4_x(const W4Params &p, cudaStream_t stream) {
+  bool taken = false;
+  cudaError_t e = cudaSuccess;
+  // the largest batch tile whose x fits in shared memory
+  if (p.M > 16) e = launch_w4_stream<XT, 4, GPT>(p, stream, &taken);
+  if (!taken && e == cudaSuccess && p.M > 8) e = launch_w4_stream<XT, 2, GPT>(p, stream, &taken);
+  if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 1, GPT>(p, stream, &taken);
+  if (taken || e != cudaSuccess) return e;
+  return p.M <= 8 ? launch_w4_direct<XT, 1, GPT>(p, stream) : launch_w4_direct<XT, 4, GPT>(p, stream);
+}
+
+template <typename XT>
+cudaError_t launch_w4_g(const W4Params &p, int group, cudaStream_t stream) {
+  return group == 128 ? launch_w4_x<XT, 1>(p, stream)
+                      : group == 64 ? launch_w4_x<XT, 2>(p, stream) : launch_w4_x<XT, 4>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_linear_w4(const m3_w4_args &a, cudaStream_t stream) {
+  W4Params p = {};
+  p.M = a.M, p.N = a.N, p.K = a.K;
+  p.tiles = (int)(((int64_t)a.K + M3_W4_TILE - 1) / M3_W4_TILE);
+  p.blocks = (int)(((int64_t)a.N + M3_W4_ROWS - 1) / M3_W4_ROWS);
+  p.x = a.x, p.ldx = a.ldx;
+  const int es = a.x_dtype == M3_BF16 ? 2 : 4;
+  p.x_vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx * es % 16 == 0;
+  p.codes = reinterpret_cast<const uint4 *>(a.codes);
+  p.scales = a.scales, p.s_ld = a.scale_stride, p.s_bf16 = a.s_dtype == M3_BF16;
+  p.groups = (int)(((int64_t)a.K + a.group - 1) / a.group);
+  p.zeros = a.zeros, p.z_ld = a.zero_stride;
+  p.y = a.y, p.ldy = a.ldy, p.y_bf16 = a.y_dtype == M3_BF16;
+  return a.x_dtype == M3_BF16 ? launch_w4_g<__nv_bfloat16>(p, a.group, stream)
+                              : launch_w4_g<float>(p, a.group, stream);
+}
+
+}  // namespace m3

@@ -1,4 +1,5 @@
-"""ctypes binding of the sm_100a decode library (include/mamba3_b200.h).
+"""ctypes binding of the sm_100a decode library (include/mamba3_b200.h,
+include/mamba3_b200_lm.h).
 
 The library is the only compute path of the CUDA backends: when it is
 missing or cannot be loaded every CUDA entry point raises instead of falling
@@ -16,8 +17,9 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
-from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -74,6 +76,13 @@ class StepArgs(ctypes.Structure):
                 ("ssm_state", c_void_p), ("bx_prev", c_void_p), ("angle_state", c_void_p),
                 ("out", c_void_p), ("out_stride_b", c_int64),
                 ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+# Argument blocks of include/mamba3_b200_lm.h, packed per call: field order,
+# types and alignment are the C structs'.  ``pack`` of a dozen numbers costs
+# the host about a tenth of filling a ctypes.Structure field by field.
+W4_ARGS = struct.Struct("@iiiiPqiPPqiPqPqi0P")        # m3_w4_args
+LOGITS_ARGS = struct.Struct("@iiiiPqPqPPiiiiPPPffffPqPqPqiiPPPPP")  # m3_logits_args
 
 
 ENTRY_POINTS = {
@@ -137,6 +146,10 @@ def load(path: str = LIB_PATH):
         lib.m3_siso_step.restype = c_int
         lib.m3_mimo_step_static.argtypes = [POINTER(Dims), POINTER(StepArgs), c_void_p]
         lib.m3_mimo_step_static.restype = c_int
+        for name in ("m3_linear_w4", "m3_process_logits", "m3_next_tokens"):
+            fn = getattr(lib, name)
+            fn.argtypes = [c_char_p, c_void_p]  # a packed argument block
+            fn.restype = c_int
         lib.m3_device_error.argtypes = [c_int]
         lib.m3_device_error.restype = c_int
         lib.m3_selftest_wait_timeout.argtypes = [c_void_p]
@@ -189,6 +202,20 @@ def require_cuda_available(what: str = "the CUDA decode backend") -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call(name: str, args: bytes, device: torch.device) -> None:
+    """Call the entry point ``name`` with a packed argument block on the
+    current stream of ``device``, made current if it is not."""
+    fn = getattr(_lib or load(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        st = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with device_guard(device):
+            st = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if st != M3_OK:
+        check(st, name)
 
 
 class device_guard:

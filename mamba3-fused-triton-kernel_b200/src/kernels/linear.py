@@ -16,7 +16,8 @@ from 32 rows cuBLAS is faster); with ``TC_ROUTE`` set, bf16 batches up to
 of SMs sharing each batch tile, ``cta_group::2``); everything else uses
 cuBLAS through ``torch.nn.functional.linear``.  ``TC_ROUTE`` is off: at the
 decode shapes measured on B200 cuBLAS is faster (24 layers of in_proj +
-out_proj at batch 256, d_model 2048: 473 us against 860 us).
+out_proj at batch 256, d_model 2048: 473 us against 860 us).  A 4-bit
+weight (``W4Weight``) always runs ``m3_linear_w4``.
 """
 
 from __future__ import annotations
@@ -27,6 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from src import _native as nat
+from src.kernels.linear_w4 import W4Weight, linear_w4
 
 SMALL_M_MAX = 256  # batch rows up to which the latency-optimised kernel is used
 TC_MAX_M = 512     # bf16 batch rows up to which TC_ROUTE uses the tcgen05 GEMM
@@ -182,8 +184,11 @@ def linear_bf16_skinny(x: torch.Tensor, weight: torch.Tensor, out_dtype=torch.bf
     return out
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    """``x @ weight.T`` for x (M, K), weight (N, K)."""
+def linear(x: torch.Tensor, weight) -> torch.Tensor:
+    """``x @ weight.T`` for x (M, K), weight (N, K); the weight may be a
+    ``W4Weight``."""
+    if isinstance(weight, W4Weight):
+        return linear_w4(x, weight.codes, weight.scales, weight.zeros, group_size=weight.group_size)
     if x.dim() == 2 and x.shape[0] <= SKINNY_ROUTE_M and uses_skinny_bf16(x, weight):
         return linear_bf16_skinny(x, weight)
     if TC_ROUTE and uses_tc_bf16(x, weight):

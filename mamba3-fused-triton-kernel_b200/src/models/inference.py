@@ -39,6 +39,10 @@ this package.  Differences from the reference, all deliberate:
   (the reference stacks the same static buffer seq_len times).
 * ``use_single_launch`` (an extra keyword, default True) selects the
   single-launch step kernel for the full-fused backend where it applies.
+* ``w4_group_size`` (an extension; 32, 64 or 128) holds both projections of
+  the full-fused backend in 4 bits with a scale per row and group of columns
+  (src.kernels.linear_w4): the weights a step streams shrink to about a
+  quarter of bf16.
 * ``step_host`` (an extension) runs a step from and to pinned host memory.
 """
 
@@ -50,6 +54,7 @@ import torch.nn.functional as F
 from src import _native
 from src.kernels import _launch
 from src.kernels.linear import linear
+from src.kernels.linear_w4 import W4Projection
 from src.kernels.mimo_decode import mamba3_mimo_decode_triton
 from src.kernels.mimo_decode_fused import mamba3_mimo_decode_fused_triton
 from src.kernels.siso_decode import mamba3_siso_decode_triton
@@ -106,7 +111,7 @@ class Mamba3Decoder:
     def __init__(self, model: Mamba3, use_triton: bool = True, use_cuda_graph: bool = False,
                  use_compile: bool = False, use_triton_fused: bool = False,
                  use_compile_cuda_graph: bool = False, use_triton_full_fused: bool = False,
-                 use_single_launch: bool = True):
+                 use_single_launch: bool = True, w4_group_size: int | None = None):
         self.model = model
         # Flag resolution as in the reference (src/models/inference.py:52-57),
         # minus the silent CPU fallback.
@@ -137,6 +142,13 @@ class Mamba3Decoder:
         self.use_single_launch = bool(use_single_launch)
         self._step_cache = None
         self._host_calls = 0
+        self._w4 = None
+        if w4_group_size is not None:
+            if not self.use_triton_full_fused:
+                raise ValueError("w4_group_size needs use_triton_full_fused=True")
+            self.use_single_launch = False  # that kernel streams unquantised weights
+            self._w4 = {name: W4Projection(lambda lin=getattr(model, name): lin.weight, w4_group_size)
+                        for name in ("in_proj", "out_proj")}
 
     # ------------------------------------------------------------------
     # public API
@@ -333,6 +345,11 @@ class Mamba3Decoder:
         self._fused_cache = (key, launch)
         return launch
 
+    def _projection(self, name: str):
+        """The weight a projection of the full-fused backend uses: the
+        model's, or its 4-bit form."""
+        return getattr(self.model, name).weight if self._w4 is None else self._w4[name].get()
+
     def _single_launch(self, state: dict, graph: bool = False):
         """Prepared single-launch step for this state and the current
         weights, or None where the kernel does not take the layer (or, with
@@ -358,14 +375,14 @@ class Mamba3Decoder:
             launch = self._single_launch(state, torch.cuda.is_current_stream_capturing())
             if launch is not None and launch.accepts(u):
                 return launch.run(u), state
-        zx = linear(u, m.in_proj.weight)
+        zx = linear(u, self._projection("in_proj"))
         if zx.dtype not in (torch.float32, torch.bfloat16) or zx.stride(1) != 1:
             zx = zx.float().contiguous()
         w_dtype = m.out_proj.weight.dtype
         y_dtype = w_dtype if w_dtype in (torch.float32, torch.bfloat16) else torch.float32
         y = torch.empty(u.shape[0], m.d_inner, device=u.device, dtype=y_dtype)
         self._fused_launch(state).run(zx, y)
-        out = linear(y.to(u.dtype), m.out_proj.weight)
+        out = linear(y.to(u.dtype), self._projection("out_proj"))
         return out, state
 
     def prefill(self, u: torch.Tensor, state: dict) -> tuple:
@@ -383,14 +400,14 @@ class Mamba3Decoder:
         m = self.model
         if self.use_triton_full_fused and B > 0 and L > 0:
             flat = u.reshape(B * L, u.shape[2])
-            zx = linear(flat, m.in_proj.weight)
+            zx = linear(flat, self._projection("in_proj"))
             if zx.dtype not in (torch.float32, torch.bfloat16) or zx.stride(1) != 1:
                 zx = zx.float().contiguous()
             w_dtype = m.out_proj.weight.dtype
             y_dtype = w_dtype if w_dtype in (torch.float32, torch.bfloat16) else torch.float32
             y = torch.empty(B * L, m.d_inner, device=u.device, dtype=y_dtype)
             if self._fused_launch(state).prefill(zx, y, L):
-                out = linear(y.to(u.dtype), m.out_proj.weight)
+                out = linear(y.to(u.dtype), self._projection("out_proj"))
                 return out.view(B, L, -1), state
         outs = []
         for t in range(L):

@@ -18,6 +18,13 @@ With a CUDA backend the residual add and the following norm are one kernel
 ``src.kernels.linear.linear``, and ``warmup_cuda_graph`` captures the whole
 token step -- embedding gather, all layers, the final norm and the LM head --
 in one CUDA graph.
+
+``generate`` decodes on from a prompt: after every token step the next token
+of each row is chosen on the GPU (``src.kernels.logits.next_tokens``:
+penalties for repeated tokens, a bias, a mask of allowed tokens, the largest
+logit or a draw), and fed to the next step without the host waiting.  With
+``w4_group_size`` every projection -- the layers', the MLPs' and the LM
+head's -- is held in 4 bits (``src.kernels.linear_w4``).
 """
 
 from __future__ import annotations
@@ -26,6 +33,8 @@ import torch
 import torch.nn.functional as F
 
 from src.kernels.linear import linear
+from src.kernels.linear_w4 import W4Projection
+from src.kernels.logits import next_tokens
 from src.kernels.norm import residual_rmsnorm
 from src.models.inference import Mamba3Decoder
 
@@ -33,14 +42,15 @@ from src.models.inference import Mamba3Decoder
 class Mamba3LMDecoder:
     """Decoder over a ``MambaLMHeadModel``.  ``decoder_kwargs``: the
     ``Mamba3Decoder`` backend flags, applied to every layer;
-    ``use_cuda_graph`` captures the whole token step."""
+    ``use_cuda_graph`` captures the whole token step; ``w4_group_size``
+    (32, 64 or 128; full-fused backend) holds every projection in 4 bits."""
 
-    def __init__(self, model, use_cuda_graph: bool = False, **decoder_kwargs):
+    def __init__(self, model, use_cuda_graph: bool = False, w4_group_size: int | None = None, **decoder_kwargs):
         self.model = model
         self.blocks = list(model.layers)
         if not self.blocks:
             raise ValueError("model has no layers")
-        self.layers = [Mamba3Decoder(b.mixer, **decoder_kwargs) for b in self.blocks]
+        self.layers = [Mamba3Decoder(b.mixer, w4_group_size=w4_group_size, **decoder_kwargs) for b in self.blocks]
         first = self.layers[0]
         self.cuda = first.use_triton or first.use_triton_fused or first.use_triton_full_fused or \
             first.use_compile or first.use_compile_cuda_graph
@@ -49,6 +59,14 @@ class Mamba3LMDecoder:
         self._graph_ids = None
         self._graph_logits = None
         self._graph_states = None
+        self._w4 = None
+        if w4_group_size is not None:
+            linears = [model.lm_head] + [lin for mlp in model.mlp_layers or [] for lin in (mlp.fc1, mlp.fc2)]
+            self._w4 = {lin: W4Projection(lambda lin=lin: lin.weight, w4_group_size) for lin in linears}
+
+    def _weight(self, lin):
+        """The weight of an MLP layer or the LM head, or its 4-bit form."""
+        return lin.weight if self._w4 is None else self._w4[lin].get()
 
     @property
     def vocab_size(self) -> int:
@@ -81,11 +99,11 @@ class Mamba3LMDecoder:
             o, _ = layer._graph_step_fn()(xn, st)
             if mlp is not None:
                 x, xm = residual_rmsnorm(x, o, m.mlp_norms[i].weight, m.mlp_norms[i].eps)
-                gate, val = linear(xm, mlp[i].fc1.weight).chunk(2, dim=-1)
-                o = linear((F.silu(gate) * val).contiguous(), mlp[i].fc2.weight)
+                gate, val = linear(xm, self._weight(mlp[i].fc1)).chunk(2, dim=-1)
+                o = linear((F.silu(gate) * val).contiguous(), self._weight(mlp[i].fc2))
             nrm = self._norm_after(i)
             x, xn = residual_rmsnorm(x, o, nrm.weight, nrm.eps)
-        return linear(xn, m.lm_head.weight)
+        return linear(xn, self._weight(m.lm_head))
 
     def warmup_cuda_graph(self, states: list, n_warmup: int = 3) -> None:
         """``n_warmup`` eager token steps (token id 0), then capture one token
@@ -126,3 +144,82 @@ class Mamba3LMDecoder:
                 logits, states = self.step(input_ids[:, t], states)
                 outs.append(logits.clone())
         return torch.stack(outs, dim=1), states
+
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, *, prompt_lengths: torch.Tensor | None = None,
+                 states: list | None = None, eos_token_id: int | None = None, temperature=None,
+                 seeds: torch.Tensor | None = None, **adjust) -> tuple:
+        """Continue ``input_ids`` (batch, length) by up to ``max_new_tokens``
+        a row; returns (tokens (batch, length + max_new_tokens) int64,
+        logprobs of the same shape, lengths (batch,)).
+
+        prompt_lengths  (batch,): rows with a shorter prompt, padded on the
+                 right; each goes on behind its own last token
+        states   a decode state to start from (a captured decoder: the one it
+                 was captured with); without it a new one, or the captured
+                 one set to zero
+        eos_token_id  a row that has produced it stops
+        temperature, seeds  as in ``next_tokens``; the draw of a token uses
+                 its place in the row as the position
+        adjust   ``next_tokens``' penalties, ``bias`` and ``allowed``; the
+                 prompt counts as seen, not as generated
+
+        ``lengths`` counts a row's prompt and what it produced (its
+        ``eos_token_id`` with it); places behind that hold 0, as do the
+        logprobs of the prompt.  Only the model's own vocabulary is produced,
+        not what pads it.  Needs a CUDA backend."""
+        if not self.cuda:
+            raise RuntimeError("generate needs a CUDA backend")
+        assert input_ids.is_cuda and input_ids.dim() == 2 and input_ids.shape[1] > 0, \
+            "input_ids must be a (batch, length) CUDA tensor"
+        assert max_new_tokens >= 0
+        B, L = input_ids.shape
+        dev = input_ids.device
+        vocab = self.model.config.vocab_size
+        if prompt_lengths is None:
+            prompt = torch.full((B,), L, dtype=torch.long, device=dev)
+        else:
+            assert prompt_lengths.shape == (B,) and not prompt_lengths.is_floating_point()
+            prompt = prompt_lengths.to(device=dev, dtype=torch.long)
+        total = L + max_new_tokens
+        tokens = torch.zeros(B, total, dtype=torch.long, device=dev)
+        place = torch.arange(L, device=dev)
+        tokens[:, :L] = torch.where(place < prompt[:, None], input_ids.long(), 0)
+        logprobs = torch.zeros(B, total, dtype=torch.float32, device=dev)
+        if B == 0:
+            return tokens, logprobs, prompt
+        # one look at the inputs, before the GPU sees them as indices
+        low, high, short, long = (int(v) for v in torch.stack(
+            (tokens.min(), tokens.max(), prompt.min(), prompt.max())).tolist())
+        if low < 0 or high >= vocab:
+            raise ValueError(f"input_ids must be in [0, {vocab})")
+        if short < 1 or long > L:
+            raise ValueError(f"prompt_lengths must be in [1, {L}]")
+        if eos_token_id is not None and not 0 <= eos_token_id < vocab:
+            raise ValueError(f"eos_token_id must be in [0, {vocab})")
+        if states is None:
+            if self._graph is not None:
+                states = self._graph_states
+                for st in states:
+                    for v in st.values():
+                        v.zero_()
+            else:
+                states = self.init_state(B, device=dev)
+        end = prompt + max_new_tokens
+        lengths = prompt.clone()
+        going = torch.ones(B, dtype=torch.bool, device=dev)
+        seen = torch.empty(B, dtype=torch.long, device=dev)
+        with torch.no_grad():
+            for t in range(total - 1):
+                logits, states = self.step(tokens[:, t], states)
+                if t + 1 < short:
+                    continue
+                seen.fill_(t + 1)
+                ids, lp = next_tokens(logits[:, :vocab], tokens, seen, prompt, temperature=temperature, seeds=seeds,
+                                      positions=seen if temperature is not None else None, **adjust)
+                write = going & (prompt <= t + 1) & (t + 1 < end)
+                tokens[:, t + 1] = torch.where(write, ids, tokens[:, t + 1])
+                logprobs[:, t + 1] = torch.where(write, lp, 0.0)
+                lengths += write
+                if eos_token_id is not None:
+                    going &= ~(write & (ids == eos_token_id))
+        return tokens, logprobs, lengths
