@@ -1,25 +1,29 @@
 // Logit adjustments and the choice of the next token.
 //
-// A row of V logits is read once: by a cluster of up to 8 CTAs that take a
-// slice each, 32 elements a thread, in registers from the load to the store
-// or the choice.  What bounds it is the read (and write) of the logits for
-// many rows, and the chain launch - load - combine for few.
+// A row of V logits is read once, by one CTA when the rows alone fill the
+// GPU, by several when they do not (a cluster of up to 8 where their results
+// have to meet).  What bounds it is the read (and write) of the logits for
+// many rows, and the chain launch - load - combine for few; so a thread works
+// on its own from the first load to the last, 32 logits at a time, and the
+// CTA meets once at the end.
 //
-//   * The history of a row is read once too: the cluster's CTAs share it out,
-//     and add every token into a counter of the CTA that holds its logit,
-//     through distributed shared memory (integers: the order does not
-//     matter).  A logit whose counter is 0, nearly every one, costs a share
-//     of a 16-byte load and a test.
+//   * The history of a row marks its tokens in a bitmap in shared memory and
+//     counts them in 16-bit counters (32-bit ones for more than 65,535
+//     tokens) beside it.  A counter is cleared by the token that marks it, so
+//     nothing of the vocabulary's size is swept but the bitmap, and a logit
+//     that was never seen, nearly every one, costs one bit.
 //   * Penalties, bias and mask are applied in fp32 operation by operation (no
 //     contraction), so the adjusted logit is that of the written formula.
-//   * Largest logit and sum of exponentials: per thread, CTA and cluster, the
-//     sum relative to the CTA's largest logit, joined in rank order.
-//   * A draw takes the largest z / T - log(-log u), that is the smallest
-//     e / p with e = -log u and p = exp(z / T - largest).  Only few elements
-//     can win, so all get a lower bound (e >= v = 1 - u, from the generator's
-//     upper 23 bits, times 1 / p), a thread's smallest gives an upper bound
-//     of the winner, and the elements below that (one or two a CTA) are
-//     compared in 64 bits.
+//   * Largest logit and sum of exponentials are kept per thread, the sum
+//     relative to the thread's largest, and joined in a fixed order.  Of the
+//     largest logit a thread remembers the 32 it was in; its index is looked
+//     up at the end, by the threads that hold the row's largest.
+//   * A draw takes the largest z / T - log(-log u).  Since e = -log u >= v =
+//     1 - u, z / T - log v bounds it from above, with v from the generator's
+//     upper 23 bits and in units of log 2: a multiply-add and a hardware
+//     logarithm.  Only logits whose bound reaches the best score the CTA has
+//     found so far (a float in shared memory that may be stale: it only
+//     prunes) are scored, and those are compared in 64 bits.
 #include <cuda_bf16.h>
 #include <float.h>
 #include <limits.h>
@@ -34,22 +38,22 @@ namespace m3 {
 
 namespace {
 
-constexpr int kVec = 8;                       // consecutive elements of a thread
-constexpr int kVecs = 4;                      // such runs a thread holds
-constexpr int kPer = kVec * kVecs;
-constexpr int kLogitThreads = 256;
-constexpr int kSliceMax = kLogitThreads * kPer;  // logits of a CTA at a time
+constexpr int kVec = 8;       // consecutive logits of a thread
+constexpr int kRuns = 4;      // such runs a thread loads at a time
+constexpr int kLogitThreads = 512;
 constexpr int kLogitWarps = kLogitThreads / 32;
+constexpr int kWindow = 51200;   // logits whose 16-bit counters a CTA holds: two CTAs per SM
+constexpr int kCountMax = 65535;
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum { kProcess = 0, kChoose = 1 };
+enum { kProcess = 0, kGreedy = 1, kDraw = 2 };
 
 struct LogitsParams {
   m3_logits_args a;
-  int slices;       // CTAs of a row: a cluster where they have to meet
-  int slice;        // logits of a CTA in a round, a multiple of 32
-  int rounds;
-  int history;      // counters are needed
+  int slices;  // CTAs of a row
+  int slice;   // logits of a CTA, a multiple of 32
+  int window;  // logits of a CTA at a time, a multiple of 32
+  int history, wide;  // counters are needed; of 32 bits
   int vec_in, vec_out, vec_bias;  // rows start on 16 bytes
 };
 
@@ -63,12 +67,6 @@ __device__ __forceinline__ uint32_t logits_peer(const void *smem, uint32_t rank)
                : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "r"(rank));
   return a;
 }
-__device__ __forceinline__ void peer_add(uint32_t addr, uint32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void peer_or(uint32_t addr, uint32_t v) {
-  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 __device__ __forceinline__ uint32_t peer_load(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -78,6 +76,11 @@ __device__ __forceinline__ uint32_t peer_load(uint32_t addr) {
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -99,34 +102,65 @@ struct RowNoise {
     }
     return c;
   }
-  __device__ __forceinline__ uint32_t word(uint32_t i) const {
-    const uint4 c = block(i >> 2);
-    const uint32_t w = i & 3;
-    return w == 0 ? c.x : w == 1 ? c.y : w == 2 ? c.z : c.w;
-  }
 };
 
-// Truncation of (w + 1/2) 2^-32 to 23 bits: a lower bound, short by less than 2^-23.
-__device__ __forceinline__ float noise_low(uint32_t w) { return __uint_as_float(w >> 9 | 0x3f800000u) - 1.f; }
+__device__ __forceinline__ uint32_t pick(const uint4 &c, int i) { return i == 0 ? c.x : i == 1 ? c.y : i == 2 ? c.z : c.w; }
+
+// log2 of a lower bound of (w + 1/2) 2^-32, its truncation to 23 bits
+__device__ __forceinline__ float noise_log2(uint32_t w) {
+  return log2_approx(__uint_as_float(w >> 9 | 0x3f800000u) - 1.f);
+}
 
 __device__ __noinline__ double draw_noise(uint32_t w) { return -log(-log1p(-((double)w + 0.5) * 0x1p-32)); }
 
-// Whether logit z with noise g beats `bz` with `bg` (token `bid`): by the
-// difference of the two, in 64 bits, so that large logits do not swallow the
-// noise.
-__device__ __forceinline__ bool draw_beats(float z, double g, int id, float bz, double bg, int bid, float temperature) {
-  if (bid == INT_MAX) return id != INT_MAX;
-  if (id == INT_MAX) return false;
-  const double d = ((double)z - (double)bz) / (double)temperature + (g - bg);
-  return d > 0.0 || (d == 0.0 && id < bid);
+// An element of a row with its noise; id INT_MAX: none.
+struct Drawn {
+  double g;
+  float z;
+  int id;
+};
+
+// Whether a beats b: by the difference of the two, in 64 bits, so that large
+// logits do not swallow the noise.  Of two infinite ones b stays.
+__device__ __forceinline__ bool draw_beats(const Drawn &a, const Drawn &b, float temperature) {
+  if (b.id == INT_MAX) return a.id != INT_MAX;
+  if (a.id == INT_MAX) return false;
+  const double d = ((double)a.z - (double)b.z) / (double)temperature + (a.g - b.g);
+  return d > 0.0 || (d == 0.0 && a.id < b.id);
 }
 
-struct Choice {  // of a CTA; 32-bit words for the peers
-  float top, sum;       // largest logit and the sum of exponentials relative to it
-  uint32_t noise_hi, noise_lo;  // of the best element, as a double
-  int id;               // or INT_MAX
-  float z;              // its adjusted logit
-  int nan_id;           // first NaN, or INT_MAX
+// A sum of exponentials relative to `from`, relative to `to` (at least as
+// large); equal ones, also infinite ones, leave it.
+__device__ __forceinline__ float rebase(float sum, float from, float to, float scale) {
+  return from == to ? sum : sum * exp2_approx((from - to) * scale);
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, o));
+  return v;
+}
+__device__ __forceinline__ Drawn warp_best(Drawn b, float temperature) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Drawn c = {__shfl_xor_sync(kFullMask, b.g, o), __shfl_xor_sync(kFullMask, b.z, o),
+                     __shfl_xor_sync(kFullMask, b.id, o)};
+    if (draw_beats(c, b, temperature)) b = c;
+  }
+  return b;
+}
+
+// How far below a score a bound may be computed of an element that reaches
+// it: the hardware logarithm and the product with the scale, which is at
+// most about 33 larger than the score.
+__device__ __forceinline__ float slack(float score) { return 1e-3f + 2e-6f * fabsf(score); }
+
+struct Choice {  // of a CTA, read by the cluster's first
+  float top, sum;
+  uint32_t noise_hi, noise_lo;
+  float z;
+  int id;      // or INT_MAX
+  int nan_id;  // first NaN, or INT_MAX
 };
 
 template <typename T>
@@ -180,55 +214,120 @@ __device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int
   }
 }
 
-// The CTA's smallest or largest v (NaN ignored), to every thread.
-template <bool MAX>
-__device__ __forceinline__ float cta_extreme(float v, float *scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(kFullMask, v, o);
-    v = MAX ? fmaxf(v, w) : fminf(v, w);
+// What a CTA needs to adjust its logits.
+struct Row {
+  const float *bias;
+  const uint32_t *seen;    // the window's bitmap, or NULL without a history
+  const uint32_t *counts;  // its counters
+  float rep, pres, freq;
+  int wide, vec_bias;
+
+  // count of the window's logit o
+  __device__ __forceinline__ uint32_t count(int o) const {
+    return wide ? counts[o] : counts[o >> 1] >> ((o & 1) * 16) & 0xffffu;
   }
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  // the run of n logits at e, the window's o; ok: its bits of the mask
+  __device__ __forceinline__ void adjust(float (&z)[kVec], int e, int o, int n, uint32_t ok) const {
+    if (seen) {
+      const uint32_t hit = seen[o >> 5] >> (o & 31) & 0xffu;
+      if (hit) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          if (!(hit >> i & 1u)) continue;
+          float v = z[i];
+          v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+          const uint32_t c = count(o + i);
+          if (c) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres);
+          z[i] = v;
+        }
+      }
+    }
+    if (bias) {
+      if (vec_bias && n == kVec) {
+        const float4 b0 = reinterpret_cast<const float4 *>(bias + e)[0];
+        const float4 b1 = reinterpret_cast<const float4 *>(bias + e)[1];
+        z[0] += b0.x, z[1] += b0.y, z[2] += b0.z, z[3] += b0.w;
+        z[4] += b1.x, z[5] += b1.y, z[6] += b1.z, z[7] += b1.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (i < n) z[i] += bias[e + i];
+      }
+    }
+    if (ok != 0xffu) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (!(ok >> i & 1u)) z[i] = -CUDART_INF_F;
+    }
+  }
+};
+
+// Marks and counts the history's tokens in [w0, w0 + n).
+__device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int w0, int n,
+                                             uint32_t *seen, uint32_t *counts) {
+  const m3_logits_args &a = p.a;
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const int64_t at = (int64_t)row * a.tokens_stride;
+  for (int i = tid; i < p.window / 32; i += nt) seen[i] = 0u;
   __syncthreads();
-  v = scratch[0];
-  for (int w = 1; w < (int)blockDim.x >> 5; ++w) v = MAX ? fmaxf(v, scratch[w]) : fminf(v, scratch[w]);
-  __syncthreads();  // the scratch may be written again
-  return v;
+  for (int i = tid; i < len; i += nt) {
+    const int64_t o = load_int(a.tokens, at + i, a.tokens_i64) - w0;
+    if (o < 0 || o >= n) continue;
+    if (p.wide)
+      counts[o] = 0u;
+    else
+      reinterpret_cast<uint16_t *>(counts)[o] = 0;
+    atomicOr(&seen[o >> 5], 1u << (o & 31));
+  }
+  __syncthreads();
+  for (int i = prompt + tid; i < len; i += nt) {
+    const int64_t o = load_int(a.tokens, at + i, a.tokens_i64) - w0;
+    if (o < 0 || o >= n) continue;
+    if (p.wide)
+      atomicAdd(&counts[o], 1u);
+    else
+      atomicAdd(&counts[o >> 1], 1u << ((o & 1) * 16));
+  }
+  __syncthreads();
 }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitsParams p) {
-  extern __shared__ __align__(16) uint32_t counters[];  // p.slice of them, with a history
-  __shared__ float scratch[kLogitWarps];
-  __shared__ int first[2];  // lowest index of the CTA's largest logit; of a NaN
-  __shared__ double warp_noise[kLogitWarps];
-  __shared__ int warp_id[kLogitWarps];
-  __shared__ float warp_z[kLogitWarps];
+__global__ void __launch_bounds__(kLogitThreads, MODE == kDraw ? 1 : 2) logits_kernel(const LogitsParams p) {
+  extern __shared__ __align__(16) uint32_t table[];  // bitmap and counters of a window
+  __shared__ float warp_f[kLogitWarps];
+  __shared__ Drawn warp_d[kLogitWarps];
+  __shared__ int first[2];   // lowest index of the window's largest logit; of a NaN
+  __shared__ float reached;  // a score some element of the CTA has, in units of log 2
   __shared__ Choice mine;
   const m3_logits_args &a = p.a;
-  const int tid = threadIdx.x, nt = blockDim.x;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.slices, rank = blockIdx.x % p.slices;
+  const int64_t begin = (int64_t)rank * p.slice;
+  const int lo = (int)min(begin, (int64_t)a.V), hi = (int)min(begin + p.slice, (int64_t)a.V);
+  if (MODE != kProcess && tid == 0) first[0] = first[1] = INT_MAX, reached = -CUDART_INF_F;
 
   pdl_wait();
   pdl_trigger();
   const char *logits = static_cast<const char *>(a.logits) + (int64_t)row * a.ld * sizeof(T);
   const int32_t *allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
-  const float *bias = a.bias ? a.bias + (int64_t)row * a.bias_stride : nullptr;
-  float rep = 1.f, pres = 0.f, freq = 0.f;
+  Row r = {};
+  r.bias = a.bias ? a.bias + (int64_t)row * a.bias_stride : nullptr;
+  r.wide = p.wide, r.vec_bias = p.vec_bias;
   int len = 0, prompt = 0;
   if (p.history) {
-    rep = a.repetition ? a.repetition[row] : a.repetition_value;
-    pres = a.presence ? a.presence[row] : a.presence_value;
-    freq = a.frequency ? a.frequency[row] : a.frequency_value;
+    r.rep = a.repetition ? a.repetition[row] : a.repetition_value;
+    r.pres = a.presence ? a.presence[row] : a.presence_value;
+    r.freq = a.frequency ? a.frequency[row] : a.frequency_value;
     const int64_t n = a.lengths ? load_int(a.lengths, row, a.lengths_i64) : a.T;
     const int64_t m = a.prompt_lengths ? load_int(a.prompt_lengths, row, a.prompt_i64) : 0;
     len = (int)min(max(n, (int64_t)0), (int64_t)a.T);
     prompt = (int)min(max(m, (int64_t)0), (int64_t)len);
+    if (len > 0) r.seen = table, r.counts = table + p.window / 32;
   }
   float temp = 1.f;
   bool drawn = false;
   RowNoise noise = {};
-  if (MODE == kChoose && a.sample) {
+  if (MODE == kDraw) {
     const float t = a.temperature ? a.temperature[row] : a.temperature_value;
     drawn = t > 0.f;
     if (drawn) temp = t;
@@ -237,243 +336,217 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const LogitsParam
     noise.c1 = (uint32_t)pos, noise.c2 = (uint32_t)(pos >> 32);
   }
   const float scale = fminf(kLog2e / temp, FLT_MAX);  // exponents are taken to base 2
-  float top = -CUDART_INF_F, sum = 0.f;  // the CTA's largest logit so far, this thread's sum relative to it
-  double best_g = 0.0;                   // this thread's best drawn element
-  float best_z = 0.f;
-  int best_id = INT_MAX, top_id = INT_MAX, nan_id = INT_MAX;
+  if (MODE != kProcess) __syncthreads();              // `first` and `reached` stand
 
-  const int window = p.slices * p.slice;
-  for (int round = 0; round < p.rounds; ++round) {
-    const int w0 = round * window, base = w0 + rank * p.slice;
-    if (round > 0) __syncthreads();  // the counters have been read
-    float z[kVecs][kVec];
-    uint32_t ok[kVecs];
+  // this thread's kRuns runs of the batch at window offset b0, adjusted
+  auto load = [&](float (&z)[kRuns][kVec], int w0, int wn, int b0) {
+    uint32_t ok[kRuns];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int o = (u * nt + tid) * kVec, e = base + o;
-      const int n = o < p.slice ? min(a.V - e, kVec) : 0;
+    for (int u = 0; u < kRuns; ++u) {
+      const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
+      ok[u] = 0xffu;
       if (n > 0) {
-        load_run<T>(z[u], logits, e, n, p.vec_in);
-        ok[u] = allowed ? (uint32_t)allowed[e >> 5] >> (e & 31) : 0xffu;
+        load_run<T>(z[u], logits, w0 + o, n, p.vec_in);
+        if (allowed) ok[u] = (uint32_t)allowed[(w0 + o) >> 5] >> ((w0 + o) & 31) & 0xffu;
       } else {
-        ok[u] = 0u;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) z[u][i] = -CUDART_INF_F;
       }
     }
-    if (p.history) {
-      for (int i = tid * 4; i < p.slice; i += nt * 4) *reinterpret_cast<uint4 *>(counters + i) = make_uint4(0, 0, 0, 0);
-      logits_cluster_sync();  // every counter is 0
-      const int inside = min(a.V - w0, window);
-      for (int i = rank * nt + tid; i < len; i += p.slices * nt) {
-        const int64_t id = load_int(a.tokens, (int64_t)row * a.tokens_stride + i, a.tokens_i64) - w0;
-        if (id < 0 || id >= inside) continue;
-        const uint32_t owner = (uint32_t)id / (uint32_t)p.slice;
-        const uint32_t at = logits_peer(counters + ((uint32_t)id - owner * p.slice), owner);
-        if (i >= prompt)
-          peer_add(at, 1u);
-        else
-          peer_or(at, 0x80000000u);
-      }
-      logits_cluster_sync();  // every token is counted
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) {
+      const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
+      if (n > 0) r.adjust(z[u], w0 + o, o, n, ok[u]);
     }
+  };
+
+  const int step = nt * kVec * kRuns;
+  float top = -CUDART_INF_F, sum = 0.f;  // the CTA's largest logit of the windows done; this thread's sum relative to it
+  Drawn best = {0.0, 0.f, INT_MAX};      // this thread's best drawn element
+  float best_score = -CUDART_INF_F, limit = -CUDART_INF_F;
+  int id = INT_MAX, nan_id = INT_MAX;
+  for (int w0 = lo; w0 < hi; w0 += p.window) {
+    const int wn = min(p.window, hi - w0);
+    if (r.seen) {
+      if (w0 > lo) __syncthreads();  // the table has been read
+      mark_history(p, row, len, prompt, w0, wn, table, table + p.window / 32);
+    }
+    float high = -CUDART_INF_F, mass = 0.f;  // this thread's largest of the window, the sum relative to it
+    int high_at = 0;                         // the batch it is in
+    for (int b0 = 0; b0 < wn; b0 += step) {
+      float z[kRuns][kVec];
+      load(z, w0, wn, b0);
+      if (MODE == kProcess) {
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int o = (u * nt + tid) * kVec, e = base + o;
-      const int n = o < p.slice ? min(a.V - e, kVec) : 0;
-      if (n <= 0) continue;
-      if (p.history) {
-        const uint4 c0 = *reinterpret_cast<const uint4 *>(counters + o);
-        const uint4 c1 = *reinterpret_cast<const uint4 *>(counters + o + 4);
-        if (c0.x | c0.y | c0.z | c0.w | c1.x | c1.y | c1.z | c1.w) {
-          const uint32_t c[kVec] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        for (int u = 0; u < kRuns; ++u) {
+          const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
+          if (n > 0)
+            store_run(z[u], static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
+                      a.out_dtype == M3_BF16, w0 + o, n, p.vec_out);
+        }
+        continue;
+      }
+      float m = -CUDART_INF_F;
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            if (c[i] == 0u) continue;
-            float v = z[u][i];
-            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-            const uint32_t count = c[i] & 0x7fffffffu;
-            if (count) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)count)), pres);
-            z[u][i] = v;
+      for (int u = 0; u < kRuns; ++u)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[u][i]);
+      if (m > high) mass = rebase(mass, high, m, scale), high = m, high_at = b0;
+      // nothing but NaN and -infinity so far: relative to 0, where a NaN shows
+      const float ref = high == -CUDART_INF_F ? 0.f : high;
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < kRuns; ++u)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) part[i & 1] += exp2_approx((z[u][i] - ref) * scale);
+      mass += part[0] + part[1];
+      if (MODE == kDraw && drawn) {
+        auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
+        float most = -CUDART_INF_F;
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 w = noise.block(((uint32_t)(w0 + b0 + (u * nt + tid) * kVec) >> 2) + h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, bound(z[u][4 * h + i], pick(w, i)));
           }
+        const float warp_most = warp_max(most);
+        limit = fmaxf(limit, __shfl_sync(kFullMask, *static_cast<volatile float *>(&reached), 0));
+        // (bounds and scores past fp32's range prune nothing: infinities compare as not below)
+        if (__any_sync(kFullMask, m > -CUDART_INF_F) && !(warp_most < limit - slack(limit))) {
+          // scores this thread's elements whose bound is not below `from`
+          auto score = [&](float from) {
+#pragma unroll
+            for (int u = 0; u < kRuns; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t e = (uint32_t)(w0 + b0 + (u * nt + tid) * kVec + 4 * h);
+                const uint4 w = noise.block(e >> 2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float v = z[u][4 * h + i];
+                  if (v > -CUDART_INF_F && !(bound(v, pick(w, i)) < from)) {
+                    const Drawn c = {draw_noise(pick(w, i)), v, (int)e + i};
+                    if (draw_beats(c, best, temp)) best = c;
+                  }
+                }
+              }
+            if (best.id != INT_MAX)
+              best_score = (float)(((double)best.z / (double)temp + best.g) * 1.4426950408889634);
+          };
+          // the warp's highest bound first: it raises the limit for the others
+          const int leader = __ffs(__ballot_sync(kFullMask, most == warp_most)) - 1;
+          if (lane == leader) score(most - slack(most));
+          limit = fmaxf(limit, __shfl_sync(kFullMask, best_score, leader));
+          if (!(most < limit - slack(limit))) score(limit - slack(limit));
+          limit = fmaxf(limit, warp_max(best_score));
+          if (lane == 0 && limit > *static_cast<volatile float *>(&reached))
+            *static_cast<volatile float *>(&reached) = limit;
         }
       }
-      if (bias) {
-        if (p.vec_bias && n == kVec) {
-          const float4 b0 = reinterpret_cast<const float4 *>(bias + e)[0];
-          const float4 b1 = reinterpret_cast<const float4 *>(bias + e)[1];
-          z[u][0] += b0.x, z[u][1] += b0.y, z[u][2] += b0.z, z[u][3] += b0.w;
-          z[u][4] += b1.x, z[u][5] += b1.y, z[u][6] += b1.z, z[u][7] += b1.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            if (i < n) z[u][i] += bias[e + i];
-        }
-      }
-      if (allowed) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          if (!(ok[u] >> i & 1u)) z[u][i] = -CUDART_INF_F;
-      }
-      if (MODE == kProcess)
-        store_run(z[u], static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
-                  a.out_dtype == M3_BF16, e, n, p.vec_out);
     }
     if (MODE == kProcess) continue;
 
-    float high = -CUDART_INF_F;
+    // the CTA's largest of the window, its index, and the first NaN
+    const float wm = warp_max(high);
+    if (lane == 0) warp_f[warp] = wm;
+    const int bad = __syncthreads_or(mass != mass);
+    float cta = warp_f[0];
+    for (int w = 1; w < nt >> 5; ++w) cta = fmaxf(cta, warp_f[w]);
+    const bool look = cta > top && (!drawn || cta == CUDART_INF_F);
+    if (look && high == cta) {
+      float z[kRuns][kVec];
+      load(z, w0, wn, high_at);
+      int at = INT_MAX;
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u)
+      for (int u = kRuns - 1; u >= 0; --u)
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) high = fmaxf(high, z[u][i]);
-    if (tid < 2) first[tid] = INT_MAX;
-    const float cta_high = cta_extreme<true>(high, scratch);
-    const bool raised = cta_high > top;
-    if (raised) {
-      sum = sum * exp2_approx((top - cta_high) * scale);  // 0 for the first round
-      if (top == -CUDART_INF_F) sum = 0.f;
-      top = cta_high;
+        for (int i = kVec - 1; i >= 0; --i)
+          if (z[u][i] == cta) at = w0 + high_at + (u * nt + tid) * kVec + i;
+      atomicMin(&first[0], at);
     }
-    // a round of NaN and -infinity only: relative to 0, where -infinity gives 0 and NaN shows
-    const float ref = top == -CUDART_INF_F ? 0.f : top;
-    float part = 0.f, low = CUDART_INF_F, low_q = CUDART_INF_F;
-    if (drawn) {
+    if (bad) {
+      for (int b0 = 0; b0 < wn; b0 += step) {
+        float z[kRuns][kVec];
+        load(z, w0, wn, b0);
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u) {
-        const uint32_t e = (uint32_t)(base + (u * nt + tid) * kVec);
+        for (int u = 0; u < kRuns; ++u)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 w = noise.block((e >> 2) + h);
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = (z[u][4 * h + i] - ref) * scale;
-            part += exp2_approx(x);
-            const float q = exp2_approx(-x), l = noise_low(ws[i]) * q;
-            if (l < low) low = l, low_q = q;
-          }
-        }
+          for (int i = 0; i < kVec; ++i)
+            if (z[u][i] != z[u][i]) atomicMin(&first[1], w0 + b0 + (u * nt + tid) * kVec + i);
       }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) part += exp2_approx((z[u][i] - ref) * scale);
-    }
-    sum += part;
-    // rare: the first NaN; always cheap: the first element that is the largest
-    if (part != part || (raised && high == cta_high)) {
-      int at = INT_MAX, bad = INT_MAX;
-#pragma unroll
-      for (int u = kVecs - 1; u >= 0; --u)
-#pragma unroll
-        for (int i = kVec - 1; i >= 0; --i) {
-          const int e = base + (u * nt + tid) * kVec + i;
-          if (z[u][i] == cta_high) at = e;
-          if (z[u][i] != z[u][i]) bad = e;
-        }
-      if (raised && at != INT_MAX) atomicMin(&first[0], at);
-      if (bad != INT_MAX) atomicMin(&first[1], bad);
-    }
-    if (drawn) {
-      // an upper bound of e / p of this thread's lowest element, the CTA's
-      // smallest of them, and room for the rounding of 1 / p
-      const float v_high = low / low_q + 0x1p-22f;
-      const float bound = low_q == CUDART_INF_F ? CUDART_INF_F : (v_high < 1.f ? -log1pf(-v_high) : 23.f) * low_q;
-      const float limit = cta_extreme<false>(bound, scratch) * 1.001f;
-      if (low <= limit && limit < CUDART_INF_F) {
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const int e = base + (u * nt + tid) * kVec + i;
-            const float q = exp2_approx(-((z[u][i] - ref) * scale));
-            if (!(q < CUDART_INF_F)) continue;
-            const uint32_t w = noise.word((uint32_t)e);
-            if (noise_low(w) * q <= limit) {
-              const double g = draw_noise(w);
-              if (draw_beats(z[u][i], g, e, best_z, best_g, best_id, temp)) best_g = g, best_id = e, best_z = z[u][i];
-            }
-          }
-      }
-    } else {
-      __syncthreads();
     }
     __syncthreads();
-    if (raised) top_id = first[0];
-    nan_id = min(nan_id, first[1]);
-    __syncthreads();  // `first` may be reset
+    if (look) id = first[0];
+    nan_id = first[1];
+    const float now = fmaxf(top, cta);
+    sum = rebase(sum, top, now, scale) + rebase(mass, high, now, scale);
+    top = now;
+    if (w0 + p.window < hi) {
+      __syncthreads();
+      if (tid == 0) first[0] = INT_MAX;
+      __syncthreads();
+    }
   }
   if (MODE == kProcess) return;
 
-  // the CTA's sum, in a fixed order, and its best drawn element
   sum = group_sum<32>(sum);
-  if (drawn) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double g = __shfl_xor_sync(kFullMask, best_g, o);
-      const int id = __shfl_xor_sync(kFullMask, best_id, o);
-      const float bz = __shfl_xor_sync(kFullMask, best_z, o);
-      if (draw_beats(bz, g, id, best_z, best_g, best_id, temp)) best_g = g, best_id = id, best_z = bz;
-    }
-  }
-  if ((tid & 31) == 0) {
-    scratch[tid >> 5] = sum;
-    warp_noise[tid >> 5] = best_g, warp_id[tid >> 5] = best_id, warp_z[tid >> 5] = best_z;
+  if (MODE == kDraw && drawn) best = warp_best(best, temp);
+  if (lane == 0) {
+    warp_f[warp] = sum;
+    if (MODE == kDraw) warp_d[warp] = best;
   }
   __syncthreads();
-  if (tid == 0) {
-    float s = scratch[0];
-    for (int w = 1; w < nt >> 5; ++w) s += scratch[w];
-    double g = 0.0;
-    float chosen = top;
-    int id = top_id;
-    if (drawn && top < CUDART_INF_F) {
-      g = warp_noise[0], id = warp_id[0], chosen = warp_z[0];
-      for (int w = 1; w < nt >> 5; ++w)
-        if (draw_beats(warp_z[w], warp_noise[w], warp_id[w], chosen, g, id, temp))
-          g = warp_noise[w], id = warp_id[w], chosen = warp_z[w];
+  if (warp == 0) {
+    const int nw = nt >> 5;
+    sum = group_sum<32>(lane < nw ? warp_f[lane] : 0.f);
+    Drawn c = {0.0, top, id};
+    if (MODE == kDraw && drawn && top < CUDART_INF_F)
+      c = warp_best(lane < nw ? warp_d[lane] : Drawn{0.0, 0.f, INT_MAX}, temp);
+    if (p.slices > 1 && lane == 0) {
+      const uint64_t bits = (uint64_t)__double_as_longlong(c.g);
+      mine.top = top, mine.sum = sum, mine.noise_hi = (uint32_t)(bits >> 32), mine.noise_lo = (uint32_t)bits;
+      mine.z = c.z, mine.id = c.id, mine.nan_id = nan_id;
     }
-    const uint64_t bits = (uint64_t)__double_as_longlong(g);
-    mine.top = top, mine.sum = s, mine.id = id, mine.nan_id = nan_id, mine.z = chosen;
-    mine.noise_hi = (uint32_t)(bits >> 32), mine.noise_lo = (uint32_t)bits;
+    best = c;
   }
-  logits_cluster_sync();  // every CTA's choice stands
-  if (rank == 0 && tid == 0) {
-    float all_top = -CUDART_INF_F, all_sum = 0.f, chosen = 0.f;
-    double g = 0.0;
-    int id = INT_MAX, bad = INT_MAX;
-    for (int r = 0; r < p.slices; ++r) {
-      const uint32_t at = logits_peer(&mine, (uint32_t)r);
-      const float t = __uint_as_float(peer_load(at + offsetof(Choice, top)));
-      const float s = __uint_as_float(peer_load(at + offsetof(Choice, sum)));
-      const int i = (int)peer_load(at + offsetof(Choice, id));
-      const float z = __uint_as_float(peer_load(at + offsetof(Choice, z)));
+  if (p.slices > 1) {
+    logits_cluster_sync();  // every CTA's choice stands
+    if (rank == 0 && warp == 0) {
+      const bool in = lane < p.slices;
+      const uint32_t at = logits_peer(&mine, in ? (uint32_t)lane : 0u);
+      const float t = in ? __uint_as_float(peer_load(at + offsetof(Choice, top))) : -CUDART_INF_F;
+      const float s = in ? __uint_as_float(peer_load(at + offsetof(Choice, sum))) : 0.f;
       const uint64_t bits = (uint64_t)peer_load(at + offsetof(Choice, noise_hi)) << 32 |
                             peer_load(at + offsetof(Choice, noise_lo));
-      const double rg = __longlong_as_double((long long)bits);
-      bad = min(bad, (int)peer_load(at + offsetof(Choice, nan_id)));
-      if (t > all_top) {
-        all_sum = all_top == -CUDART_INF_F ? s : all_sum * exp2f((all_top - t) * scale) + s;
-        all_top = t;
-      } else if (t > -CUDART_INF_F) {
-        all_sum += s * exp2f((t - all_top) * scale);
+      Drawn c = {__longlong_as_double((long long)bits), __uint_as_float(peer_load(at + offsetof(Choice, z))),
+                 in ? (int)peer_load(at + offsetof(Choice, id)) : INT_MAX};
+      nan_id = __reduce_min_sync(kFullMask, in ? (int)peer_load(at + offsetof(Choice, nan_id)) : INT_MAX);
+      top = warp_max(t);
+      sum = group_sum<32>(rebase(s, t, top, scale));
+      // of two infinite logits neither beats the other by the difference: the lowest index
+      if (top == CUDART_INF_F) {
+        c.id = __reduce_min_sync(kFullMask, t == top ? c.id : INT_MAX);
+        c.z = top;
+        best = c;
+      } else {
+        best = warp_best(c, temp);
       }
-      // of two infinite logits the difference is NaN: the lower rank's stays
-      if (draw_beats(z, rg, i, chosen, g, id, temp)) g = rg, id = i, chosen = z;
     }
-    float lp;
-    if (bad != INT_MAX) {
-      id = bad, lp = CUDART_NAN_F;
-    } else if (all_top == -CUDART_INF_F) {
-      id = 0, lp = -CUDART_INF_F;
-    } else {
-      lp = (chosen - all_top) / temp - logf(all_sum);  // NaN with an infinite logit, as the formula gives
-    }
-    a.ids[row] = id;
+  }
+  if (rank == 0 && tid == 0) {
+    // NaN with an infinite logit, as the formula gives
+    float lp = (best.z - top) / temp - logf(sum);
+    int chosen = best.id;
+    if (nan_id != INT_MAX)
+      chosen = nan_id, lp = CUDART_NAN_F;
+    else if (top == -CUDART_INF_F)
+      chosen = 0, lp = -CUDART_INF_F;
+    a.ids[row] = chosen;
     a.logprobs[row] = lp;
   }
-  logits_cluster_sync();  // no CTA leaves while its choice is read
+  if (p.slices > 1) logits_cluster_sync();  // no CTA leaves while its choice is read
 }
 
 bool rows_on_16(const void *p, int64_t ld, int B, int size) {
@@ -487,26 +560,33 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   p.history = a.tokens && a.T > 0 &&
               (a.repetition || a.presence || a.frequency || a.repetition_value != 1.f || a.presence_value != 0.f ||
                a.frequency_value != 0.f);
+  p.wide = a.T > kCountMax;
   p.vec_in = rows_on_16(a.logits, a.ld, a.B, sizeof(T));
   p.vec_out = a.out && rows_on_16(a.out, a.out_ld, a.B, a.out_dtype == M3_BF16 ? 2 : 4);
   p.vec_bias = a.bias && rows_on_16(a.bias, a.bias_stride, a.B, 4);
-  const bool cluster = MODE == kChoose || p.history;
-  if (cluster) {
-    p.slices = 8;
-    p.rounds = (int)(((int64_t)a.V + p.slices * kSliceMax - 1) / (p.slices * kSliceMax));
-    const int parts = p.slices * p.rounds;
-    p.slice = ((a.V + parts - 1) / parts + 31) / 32 * 32;
-  } else {  // CTAs that need not meet: enough of them for one row
-    p.slice = 2048;
-    p.slices = (a.V + p.slice - 1) / p.slice;
-    p.rounds = 1;
+  // CTAs of a row: what fills two CTAs an SM, at least one run a thread each;
+  // those that have to meet are a cluster, a power of two up to 8
+  const int fill = 2 * sm_count_current() / a.B;
+  const int runs = (int)(((int64_t)a.V + kLogitThreads * kVec - 1) / (kLogitThreads * kVec));
+  int want = max(1, min(fill, runs));
+  if (MODE != kProcess) {
+    p.slices = 1;
+    while (p.slices < 8 && p.slices * 2 <= want) p.slices *= 2;
+  } else {
+    p.slices = want;
   }
+  p.slice = (int)(((int64_t)a.V + p.slices - 1) / p.slices + 31) / 32 * 32;
+  p.window = p.history ? min(p.slice, p.wide ? kWindow / 2 : kWindow) : p.slice;
   const int64_t grid = (int64_t)a.B * p.slices;
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+  auto kern = logits_kernel<T, MODE>;
+  const size_t smem = p.history ? (size_t)p.window / 8 + (size_t)p.window * (p.wide ? 4 : 2) : 0;
+  static LaunchCache cache;
+  if (cudaError_t e = ensure_smem_optin(cache, kern, kWindow / 8 + kWindow * 2); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)((p.slice + kPer - 1) / kPer + 31) / 32 * 32);
-  cfg.dynamicSmemBytes = p.history ? (size_t)p.slice * 4 : 0;
+  cfg.blockDim = dim3((unsigned)min(kLogitThreads, ((p.slice + kVec - 1) / kVec + 31) / 32 * 32));
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -516,8 +596,8 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster ? 2 : 1;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, logits_kernel<T, MODE>, p); e != cudaSuccess) return e;
+  cfg.numAttrs = MODE != kProcess && p.slices > 1 ? 2 : 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p); e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 
@@ -529,8 +609,11 @@ cudaError_t launch_process_logits(const m3_logits_args &a, cudaStream_t stream) 
 }
 
 cudaError_t launch_next_tokens(const m3_logits_args &a, cudaStream_t stream) {
-  return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kChoose>(a, stream)
-                            : launch_logits_t<float, kChoose>(a, stream);
+  if (a.sample)
+    return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kDraw>(a, stream)
+                              : launch_logits_t<float, kDraw>(a, stream);
+  return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kGreedy>(a, stream)
+                            : launch_logits_t<float, kGreedy>(a, stream);
 }
 
 }  // namespace m3
