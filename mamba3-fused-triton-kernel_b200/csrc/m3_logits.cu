@@ -4,8 +4,8 @@
 // GPU, by several when they do not (a cluster of up to 8 where their results
 // have to meet).  What bounds it is the read (and write) of the logits for
 // many rows, and the chain launch - load - combine for few; so a thread works
-// on its own from the first load to the last, 32 logits at a time, and the
-// CTA meets once at the end.
+// on its own from the first load to the last, in runs of 8 logits with two
+// more in flight, and the CTA meets at the end.
 //
 //   * The history of a row marks its tokens in a bitmap in shared memory and
 //     counts them in 16-bit counters (32-bit ones for more than 65,535
@@ -16,14 +16,15 @@
 //     contraction), so the adjusted logit is that of the written formula.
 //   * Largest logit and sum of exponentials are kept per thread, the sum
 //     relative to the thread's largest, and joined in a fixed order.  Of the
-//     largest logit a thread remembers the 32 it was in; its index is looked
+//     largest logit a thread remembers the run it was in; its index is looked
 //     up at the end, by the threads that hold the row's largest.
 //   * A draw takes the largest z / T - log(-log u).  Since e = -log u >= v =
 //     1 - u, z / T - log v bounds it from above, with v from the generator's
 //     upper 23 bits and in units of log 2: a multiply-add and a hardware
-//     logarithm.  Only logits whose bound reaches the best score the CTA has
-//     found so far (a float in shared memory that may be stale: it only
-//     prunes) are scored, and those are compared in 64 bits.
+//     logarithm.  A thread keeps the run with its highest bound and the second
+//     highest; at the end the CTA's highest gives a score that is reached, and
+//     the few logits whose bound is not below it are scored and compared in
+//     64 bits.
 #include <cuda_bf16.h>
 #include <float.h>
 #include <limits.h>
@@ -39,7 +40,8 @@ namespace m3 {
 namespace {
 
 constexpr int kVec = 8;       // consecutive logits of a thread
-constexpr int kRuns = 4;      // such runs a thread loads at a time
+constexpr int kRuns = 2;      // such runs a thread loads at a time
+constexpr int kTokens = 4;    // tokens of the history a thread holds
 constexpr int kLogitThreads = 512;
 constexpr int kLogitWarps = kLogitThreads / 32;
 constexpr int kWindow = 51200;   // logits whose 16-bit counters a CTA holds: two CTAs per SM
@@ -163,32 +165,40 @@ struct Choice {  // of a CTA, read by the cluster's first
   int nan_id;  // first NaN, or INT_MAX
 };
 
+// A run as it lies in memory; logits past the row's end are -infinity.
 template <typename T>
-__device__ __forceinline__ void load_run(float (&z)[kVec], const void *row, int e, int n, int vec) {
-  const T *p = static_cast<const T *>(row) + e;
-  if (vec && n == kVec) {
-    if (sizeof(T) == 2) {
-      const uint4 q = *reinterpret_cast<const uint4 *>(p);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+struct Run {
+  static constexpr int kWords = sizeof(T) * kVec / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void *row, int e, int n, int vec) {
+    const T *p = static_cast<const T *>(row) + e;
+    if (vec && n >= kVec) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        z[2 * i] = __uint_as_float(w[i] << 16);
-        z[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 q = reinterpret_cast<const uint4 *>(p)[i];
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
       }
-    } else {
-      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-      z[0] = a.x, z[1] = a.y, z[2] = a.z, z[3] = a.w, z[4] = b.x, z[5] = b.y, z[6] = b.z, z[7] = b.w;
-    }
-    return;
-  }
+    } else if (sizeof(T) == 2) {
+      const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) z[i] = i < n ? (float)p[i] : -CUDART_INF_F;
-}
+      for (int i = 0; i < kWords; ++i)
+        w[i] = (2 * i < n ? h[2 * i] : 0xff80u) | (uint32_t)(2 * i + 1 < n ? h[2 * i + 1] : 0xff80u) << 16;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0xff800000u;
+    }
+  }
+  __device__ __forceinline__ void get(float (&z)[kVec]) const {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      z[i] = __uint_as_float(sizeof(T) == 2 ? (i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) : w[i % kWords]);
+  }
+};
 
 __device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int bf16, int e, int n, int vec) {
   if (bf16) {
     __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(row) + e;
-    if (vec && n == kVec) {
+    if (vec && n >= kVec) {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -203,7 +213,7 @@ __device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int
     }
   } else {
     float *p = static_cast<float *>(row) + e;
-    if (vec && n == kVec) {
+    if (vec && n >= kVec) {
       reinterpret_cast<float4 *>(p)[0] = make_float4(z[0], z[1], z[2], z[3]);
       reinterpret_cast<float4 *>(p)[1] = make_float4(z[4], z[5], z[6], z[7]);
     } else {
@@ -243,7 +253,7 @@ struct Row {
       }
     }
     if (bias) {
-      if (vec_bias && n == kVec) {
+      if (vec_bias && n >= kVec) {
         const float4 b0 = reinterpret_cast<const float4 *>(bias + e)[0];
         const float4 b1 = reinterpret_cast<const float4 *>(bias + e)[1];
         z[0] += b0.x, z[1] += b0.y, z[2] += b0.z, z[3] += b0.w;
@@ -262,59 +272,74 @@ struct Row {
   }
 };
 
-// Marks and counts the history's tokens in [w0, w0 + n).
+// Marks and counts the history's tokens in [w0, w0 + n); held: the first
+// kTokens of every thread, read already (-1: not in the vocabulary).
 __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int w0, int n,
-                                             uint32_t *seen, uint32_t *counts) {
+                                             const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
   const m3_logits_args &a = p.a;
   const int tid = threadIdx.x, nt = blockDim.x;
   const int64_t at = (int64_t)row * a.tokens_stride;
-  for (int i = tid; i < p.window / 32; i += nt) seen[i] = 0u;
-  __syncthreads();
-  for (int i = tid; i < len; i += nt) {
-    const int64_t o = load_int(a.tokens, at + i, a.tokens_i64) - w0;
-    if (o < 0 || o >= n) continue;
+  auto mark = [&](int64_t o) {
+    if (o < 0 || o >= n) return;
     if (p.wide)
       counts[o] = 0u;
     else
       reinterpret_cast<uint16_t *>(counts)[o] = 0;
     atomicOr(&seen[o >> 5], 1u << (o & 31));
-  }
-  __syncthreads();
-  for (int i = prompt + tid; i < len; i += nt) {
-    const int64_t o = load_int(a.tokens, at + i, a.tokens_i64) - w0;
-    if (o < 0 || o >= n) continue;
+  };
+  auto count = [&](int64_t o) {
+    if (o < 0 || o >= n) return;
     if (p.wide)
       atomicAdd(&counts[o], 1u);
     else
       atomicAdd(&counts[o >> 1], 1u << ((o & 1) * 16));
-  }
+  };
+  const int rest = kTokens * nt + tid;  // the thread's first token that is not held
+  for (int i = tid; i < p.window / 32; i += nt) seen[i] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k)
+    if (tid + k * nt < len) mark(held[k] - w0);
+  for (int i = rest; i < len; i += nt) mark(load_int(a.tokens, at + i, a.tokens_i64) - w0);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k)
+    if (tid + k * nt < len && tid + k * nt >= prompt) count(held[k] - w0);
+  for (int i = rest; i < len; i += nt)
+    if (i >= prompt) count(load_int(a.tokens, at + i, a.tokens_i64) - w0);
   __syncthreads();
 }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kLogitThreads, MODE == kDraw ? 1 : 2) logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsParams p) {
   extern __shared__ __align__(16) uint32_t table[];  // bitmap and counters of a window
-  __shared__ float warp_f[kLogitWarps];
+  __shared__ float warp_f[kLogitWarps], warp_b[kLogitWarps];
   __shared__ Drawn warp_d[kLogitWarps];
   __shared__ int first[2];   // lowest index of the window's largest logit; of a NaN
-  __shared__ float reached;  // a score some element of the CTA has, in units of log 2
+  __shared__ float reached;  // a score some element of the window reaches, in units of log 2
   __shared__ Choice mine;
   const m3_logits_args &a = p.a;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.slices, rank = blockIdx.x % p.slices;
   const int64_t begin = (int64_t)rank * p.slice;
   const int lo = (int)min(begin, (int64_t)a.V), hi = (int)min(begin + p.slice, (int64_t)a.V);
-  if (MODE != kProcess && tid == 0) first[0] = first[1] = INT_MAX, reached = -CUDART_INF_F;
+  if (MODE != kProcess && tid == 0) first[0] = first[1] = INT_MAX;
 
   pdl_wait();
   pdl_trigger();
   const char *logits = static_cast<const char *>(a.logits) + (int64_t)row * a.ld * sizeof(T);
   const int32_t *allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
   Row r = {};
-  r.bias = a.bias ? a.bias + (int64_t)row * a.bias_stride : nullptr;
-  r.wide = p.wide, r.vec_bias = p.vec_bias;
-  int len = 0, prompt = 0;
+  int len = 0, prompt = 0, held[kTokens];
   if (p.history) {
+    // the tokens first, whatever the length turns out to be
+    const int64_t at = (int64_t)row * a.tokens_stride;
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int i = tid + k * nt;
+      const int64_t t = i < a.T ? load_int(a.tokens, at + i, a.tokens_i64) : -1;
+      held[k] = t >= 0 && t < a.V ? (int)t : -1;
+    }
     r.rep = a.repetition ? a.repetition[row] : a.repetition_value;
     r.pres = a.presence ? a.presence[row] : a.presence_value;
     r.freq = a.frequency ? a.frequency[row] : a.frequency_value;
@@ -324,6 +349,8 @@ __global__ void __launch_bounds__(kLogitThreads, MODE == kDraw ? 1 : 2) logits_k
     prompt = (int)min(max(m, (int64_t)0), (int64_t)len);
     if (len > 0) r.seen = table, r.counts = table + p.window / 32;
   }
+  r.bias = a.bias ? a.bias + (int64_t)row * a.bias_stride : nullptr;
+  r.wide = p.wide, r.vec_bias = p.vec_bias;
   float temp = 1.f;
   bool drawn = false;
   RowNoise noise = {};
@@ -336,146 +363,155 @@ __global__ void __launch_bounds__(kLogitThreads, MODE == kDraw ? 1 : 2) logits_k
     noise.c1 = (uint32_t)pos, noise.c2 = (uint32_t)(pos >> 32);
   }
   const float scale = fminf(kLog2e / temp, FLT_MAX);  // exponents are taken to base 2
-  if (MODE != kProcess) __syncthreads();              // `first` and `reached` stand
+  auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
+  if (MODE != kProcess) __syncthreads();  // `first` stands
 
-  // this thread's kRuns runs of the batch at window offset b0, adjusted
-  auto load = [&](float (&z)[kRuns][kVec], int w0, int wn, int b0) {
-    uint32_t ok[kRuns];
-#pragma unroll
-    for (int u = 0; u < kRuns; ++u) {
-      const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
-      ok[u] = 0xffu;
-      if (n > 0) {
-        load_run<T>(z[u], logits, w0 + o, n, p.vec_in);
-        if (allowed) ok[u] = (uint32_t)allowed[(w0 + o) >> 5] >> ((w0 + o) & 31) & 0xffu;
-      } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) z[u][i] = -CUDART_INF_F;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kRuns; ++u) {
-      const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
-      if (n > 0) r.adjust(z[u], w0 + o, o, n, ok[u]);
-    }
+  auto fetch = [&](Run<T> &q, uint32_t &ok, int e, int n) {
+    if (n <= 0) return;
+    q.load(logits, e, n, p.vec_in);
+    ok = allowed ? (uint32_t)allowed[e >> 5] >> (e & 31) & 0xffu : 0xffu;
+  };
+  // the run at window offset o, adjusted (again, for a closer look)
+  auto look_at = [&](float (&z)[kVec], int w0, int wn, int o) {
+    Run<T> q;
+    uint32_t ok = 0u;
+    fetch(q, ok, w0 + o, wn - o);
+    q.get(z);
+    r.adjust(z, w0 + o, o, wn - o, ok);
   };
 
-  const int step = nt * kVec * kRuns;
+  const int step = nt * kVec;
   float top = -CUDART_INF_F, sum = 0.f;  // the CTA's largest logit of the windows done; this thread's sum relative to it
   Drawn best = {0.0, 0.f, INT_MAX};      // this thread's best drawn element
-  float best_score = -CUDART_INF_F, limit = -CUDART_INF_F;
   int id = INT_MAX, nan_id = INT_MAX;
   for (int w0 = lo; w0 < hi; w0 += p.window) {
     const int wn = min(p.window, hi - w0);
+    Run<T> next[kRuns];
+    uint32_t next_ok[kRuns];
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) fetch(next[u], next_ok[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
     if (r.seen) {
       if (w0 > lo) __syncthreads();  // the table has been read
-      mark_history(p, row, len, prompt, w0, wn, table, table + p.window / 32);
+      mark_history(p, row, len, prompt, w0, wn, held, table, table + p.window / 32);
     }
     float high = -CUDART_INF_F, mass = 0.f;  // this thread's largest of the window, the sum relative to it
-    int high_at = 0;                         // the batch it is in
-    for (int b0 = 0; b0 < wn; b0 += step) {
-      float z[kRuns][kVec];
-      load(z, w0, wn, b0);
-      if (MODE == kProcess) {
+    int high_at = 0;                         // the run it is in
+    if (MODE == kDraw && tid == 0) reached = -CUDART_INF_F;
+    float most = -CUDART_INF_F, second = -CUDART_INF_F;  // highest bounds of its runs
+    int most_at = -1;
+    for (int o0 = tid * kVec; o0 < wn; o0 += kRuns * step) {
 #pragma unroll
-        for (int u = 0; u < kRuns; ++u) {
-          const int o = b0 + (u * nt + tid) * kVec, n = min(wn - o, kVec);
-          if (n > 0)
-            store_run(z[u], static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
-                      a.out_dtype == M3_BF16, w0 + o, n, p.vec_out);
+      for (int u = 0; u < kRuns; ++u) {
+        const int o = o0 + u * step, n = wn - o;
+        if (n <= 0) continue;
+        float z[kVec];
+        next[u].get(z);
+        const uint32_t ok = next_ok[u];
+        fetch(next[u], next_ok[u], w0 + o + kRuns * step, n - kRuns * step);
+        r.adjust(z, w0 + o, o, n, ok);
+        if (MODE == kProcess) {
+          store_run(z, static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
+                    a.out_dtype == M3_BF16, w0 + o, n, p.vec_out);
+          continue;
         }
-        continue;
-      }
-      float m = -CUDART_INF_F;
+        float m = -CUDART_INF_F;
 #pragma unroll
-      for (int u = 0; u < kRuns; ++u)
+        for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[i]);
+        if (m > high) mass = rebase(mass, high, m, scale), high = m, high_at = o;
+        // nothing but NaN and -infinity so far: relative to 0, where a NaN shows
+        const float ref = high == -CUDART_INF_F ? 0.f : high;
+        float part[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) m = fmaxf(m, z[u][i]);
-      if (m > high) mass = rebase(mass, high, m, scale), high = m, high_at = b0;
-      // nothing but NaN and -infinity so far: relative to 0, where a NaN shows
-      const float ref = high == -CUDART_INF_F ? 0.f : high;
-      float part[2] = {0.f, 0.f};
+        for (int i = 0; i < kVec; ++i) part[i & 1] += exp2_approx((z[i] - ref) * scale);
+        mass += part[0] + part[1];
+        if (MODE == kDraw && drawn) {
+          float b = -CUDART_INF_F;
 #pragma unroll
-      for (int u = 0; u < kRuns; ++u)
+          for (int h = 0; h < kVec / 4; ++h) {
+            const uint4 w = noise.block(((uint32_t)(w0 + o) >> 2) + h);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) part[i & 1] += exp2_approx((z[u][i] - ref) * scale);
-      mass += part[0] + part[1];
-      if (MODE == kDraw && drawn) {
-        auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
-        float most = -CUDART_INF_F;
-#pragma unroll
-        for (int u = 0; u < kRuns; ++u)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w = noise.block(((uint32_t)(w0 + b0 + (u * nt + tid) * kVec) >> 2) + h);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most = fmaxf(most, bound(z[u][4 * h + i], pick(w, i)));
+            for (int i = 0; i < 4; ++i) b = fmaxf(b, bound(z[4 * h + i], pick(w, i)));
           }
-        const float warp_most = warp_max(most);
-        limit = fmaxf(limit, __shfl_sync(kFullMask, *static_cast<volatile float *>(&reached), 0));
-        // (bounds and scores past fp32's range prune nothing: infinities compare as not below)
-        if (__any_sync(kFullMask, m > -CUDART_INF_F) && !(warp_most < limit - slack(limit))) {
-          // scores this thread's elements whose bound is not below `from`
-          auto score = [&](float from) {
-#pragma unroll
-            for (int u = 0; u < kRuns; ++u)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t e = (uint32_t)(w0 + b0 + (u * nt + tid) * kVec + 4 * h);
-                const uint4 w = noise.block(e >> 2);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float v = z[u][4 * h + i];
-                  if (v > -CUDART_INF_F && !(bound(v, pick(w, i)) < from)) {
-                    const Drawn c = {draw_noise(pick(w, i)), v, (int)e + i};
-                    if (draw_beats(c, best, temp)) best = c;
-                  }
-                }
-              }
-            if (best.id != INT_MAX)
-              best_score = (float)(((double)best.z / (double)temp + best.g) * 1.4426950408889634);
-          };
-          // the warp's highest bound first: it raises the limit for the others
-          const int leader = __ffs(__ballot_sync(kFullMask, most == warp_most)) - 1;
-          if (lane == leader) score(most - slack(most));
-          limit = fmaxf(limit, __shfl_sync(kFullMask, best_score, leader));
-          if (!(most < limit - slack(limit))) score(limit - slack(limit));
-          limit = fmaxf(limit, warp_max(best_score));
-          if (lane == 0 && limit > *static_cast<volatile float *>(&reached))
-            *static_cast<volatile float *>(&reached) = limit;
+          // of bounds past fp32's range too the last run is kept
+          if (b >= most)
+            second = most, most = b, most_at = o;
+          else
+            second = fmaxf(second, b);
         }
       }
     }
     if (MODE == kProcess) continue;
 
     // the CTA's largest of the window, its index, and the first NaN
-    const float wm = warp_max(high);
-    if (lane == 0) warp_f[warp] = wm;
+    const float warp_high = warp_max(high), warp_most = MODE == kDraw ? warp_max(most) : 0.f;
+    if (lane == 0) warp_f[warp] = warp_high, warp_b[warp] = warp_most;
     const int bad = __syncthreads_or(mass != mass);
     float cta = warp_f[0];
     for (int w = 1; w < nt >> 5; ++w) cta = fmaxf(cta, warp_f[w]);
     const bool look = cta > top && (!drawn || cta == CUDART_INF_F);
     if (look && high == cta) {
-      float z[kRuns][kVec];
-      load(z, w0, wn, high_at);
+      float z[kVec];
+      look_at(z, w0, wn, high_at);
       int at = INT_MAX;
 #pragma unroll
-      for (int u = kRuns - 1; u >= 0; --u)
-#pragma unroll
-        for (int i = kVec - 1; i >= 0; --i)
-          if (z[u][i] == cta) at = w0 + high_at + (u * nt + tid) * kVec + i;
+      for (int i = kVec - 1; i >= 0; --i)
+        if (z[i] == cta) at = w0 + high_at + i;
       atomicMin(&first[0], at);
     }
     if (bad) {
-      for (int b0 = 0; b0 < wn; b0 += step) {
-        float z[kRuns][kVec];
-        load(z, w0, wn, b0);
+      for (int o = tid * kVec; o < wn; o += step) {
+        float z[kVec];
+        look_at(z, w0, wn, o);
 #pragma unroll
-        for (int u = 0; u < kRuns; ++u)
-#pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            if (z[u][i] != z[u][i]) atomicMin(&first[1], w0 + b0 + (u * nt + tid) * kVec + i);
+        for (int i = 0; i < kVec; ++i)
+          if (z[i] != z[i]) atomicMin(&first[1], w0 + o + i);
       }
+    }
+    if (MODE == kDraw && drawn && cta > -CUDART_INF_F) {
+      // scores the run's elements whose bound is not below `from`
+      auto score = [&](int o, float from) {
+        float z[kVec];
+        look_at(z, w0, wn, o);
+#pragma unroll 1
+        for (int h = 0; h < kVec / 4; ++h) {
+          const uint32_t e = (uint32_t)(w0 + o + 4 * h);
+          const uint4 w = noise.block(e >> 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = h ? z[4 + i] : z[i];
+            if (v > -CUDART_INF_F && !(bound(v, pick(w, i)) < from)) {
+              const Drawn c = {draw_noise(pick(w, i)), v, (int)e + i};
+              if (draw_beats(c, best, temp)) best = c;
+            }
+          }
+        }
+      };
+      float cta_most = warp_b[0];
+      for (int w = 1; w < nt >> 5; ++w) cta_most = fmaxf(cta_most, warp_b[w]);
+      if (most_at >= 0 && most == cta_most) {
+        // bounds and scores past fp32's range prune nothing: infinities compare as not below
+        float z[kVec], low = -CUDART_INF_F;
+        look_at(z, w0, wn, most_at);
+#pragma unroll
+        for (int h = 0; h < kVec / 4; ++h) {
+          const uint4 w = noise.block(((uint32_t)(w0 + most_at) >> 2) + h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (bound(z[4 * h + i], pick(w, i)) == most) {
+              // e for v rounded up to the next of the 23 bits; at most 23
+              const float v = __uint_as_float(pick(w, i) >> 9 | 0x3f800000u) - 1.f + 0x1p-23f;
+              const float e = v < 1.f ? -log1pf(-v) : 23.f;
+              low = fmaf(z[4 * h + i], scale, -log2_approx(e));
+            }
+        }
+        reached = low;
+      }
+      __syncthreads();
+      const float limit = reached - slack(reached);
+      if (most_at >= 0 && !(most < limit)) score(most_at, limit);
+      if (!(second < limit))
+        for (int o = tid * kVec; o < wn; o += step)
+          if (o != most_at) score(o, limit);
     }
     __syncthreads();
     if (look) id = first[0];

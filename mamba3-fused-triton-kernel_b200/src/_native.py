@@ -92,6 +92,7 @@ ENTRY_POINTS = {
 }
 
 _lib = None
+_packed: dict = {}  # entry points that take a packed argument block
 _lock = threading.Lock()
 
 
@@ -204,15 +205,16 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call(name: str, args: bytes, device: torch.device) -> None:
+def call(name: str, args: bytes, index: int) -> None:
     """Call the entry point ``name`` with a packed argument block on the
-    current stream of ``device``, made current if it is not."""
-    fn = getattr(_lib or load(), name)
-    index = device.index
-    if torch.cuda.current_device() == index:
+    current stream of CUDA device ``index``, made current if it is not."""
+    fn = _packed.get(name)
+    if fn is None:
+        fn = _packed[name] = getattr(load(), name)
+    if torch._C._cuda_getDevice() == index:
         st = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with device_guard(device):
+        with device_guard(torch.device("cuda", index)):
             st = fn(args, torch._C._cuda_getCurrentRawStream(index))
     if st != M3_OK:
         check(st, name)

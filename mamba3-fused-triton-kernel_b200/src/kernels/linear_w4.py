@@ -189,38 +189,47 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     the scale.  Inference only: x with a gradient is refused."""
     if group_size not in GROUP_SIZES:
         _check_group(group_size)
-    assert x.is_cuda and x.dim() == 2, "x must be a (M, K) CUDA tensor"
+    dev = x.get_device() if x.is_cuda else -1
+    assert dev >= 0 and x.dim() == 2, "x must be a (M, K) CUDA tensor"
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("linear_w4 has no gradient: call it under torch.no_grad() or on x.detach()")
     M, K = x.shape
     N, groups = scales.shape
     dtype = x.dtype
-    out_dtype = dtype if out_dtype is None else out_dtype
+    if out_dtype is None:
+        out_dtype = dtype
     x_code, s_code, y_code = _CODE.get(dtype), _CODE.get(scales.dtype), _CODE.get(out_dtype)
     assert x_code is not None and s_code is not None and y_code is not None, \
         f"x, scales and out_dtype must be float32 or bfloat16 (got {dtype}, {scales.dtype}, {out_dtype})"
     assert K > 0 and N > 0, "linear_w4 needs at least one row and one column of weight"
-    blocks = (-(-N // ROWS), -(-K // TILE), ROWS, 16)
-    assert codes.dtype == torch.int32 and codes.shape == blocks and codes.is_contiguous(), \
+    blocks = ((N + ROWS - 1) // ROWS, (K + TILE - 1) // TILE, ROWS, 16)
+    assert codes.shape == blocks and codes.dtype == torch.int32 and codes.is_contiguous(), \
         f"codes must be contiguous int32 {blocks}, got {codes.dtype} {tuple(codes.shape)}"
-    assert groups == -(-K // group_size), f"scales must be {(N, -(-K // group_size))}, got {tuple(scales.shape)}"
-    dev = x.device
-    assert codes.device == dev and scales.device == dev, f"all tensors must be on {dev}"
-    scales = _rows(scales)
+    assert groups == (K + group_size - 1) // group_size, \
+        f"scales must be {(N, -(-K // group_size))}, got {tuple(scales.shape)}"
+    assert codes.get_device() == dev and scales.get_device() == dev, f"all tensors must be on {x.device}"
+    if scales.is_contiguous():
+        s_pitch = groups
+    else:
+        scales = _rows(scales)
+        s_pitch = _pitch(scales)
     z_ptr = z_pitch = 0
     if zeros is not None:
-        assert zeros.dtype == torch.uint8 and zeros.shape == (N, groups) and zeros.device == dev, \
-            f"zeros must be uint8 {(N, groups)} on {dev}, got {zeros.dtype} {tuple(zeros.shape)} on {zeros.device}"
+        assert zeros.dtype == torch.uint8 and zeros.shape == (N, groups) and zeros.get_device() == dev, \
+            f"zeros must be uint8 {(N, groups)} on {x.device}, got {zeros.dtype} {tuple(zeros.shape)} on {zeros.device}"
         zeros = _rows(zeros)
         z_ptr, z_pitch = zeros.data_ptr(), _pitch(zeros)
-    y = x.new_empty((M, N), dtype=out_dtype)
-    if M == 0:
-        return y
-    if K > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    nat.call("m3_linear_w4", nat.W4_ARGS.pack(
-        M, N, K, group_size, x.data_ptr(), x.stride(0), x_code, codes.data_ptr(), scales.data_ptr(), _pitch(scales),
-        s_code, z_ptr, z_pitch, y.data_ptr(), N, y_code), dev)
+    if x.is_contiguous():
+        ldx = K
+    else:
+        if x.stride(1) != 1 and K > 1:
+            x = x.contiguous()
+        ldx = x.stride(0)
+    y = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    if M > 0:
+        nat.call("m3_linear_w4", nat.W4_ARGS.pack(
+            M, N, K, group_size, x.data_ptr(), ldx, x_code, codes.data_ptr(), scales.data_ptr(), s_pitch, s_code,
+            z_ptr, z_pitch, y.data_ptr(), N, y_code), dev)
     return y
 
 

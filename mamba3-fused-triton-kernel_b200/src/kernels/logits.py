@@ -25,94 +25,106 @@ import torch
 from src import _native as nat
 
 _CODE = {torch.float32: nat.M3_F32, torch.bfloat16: nat.M3_BF16}
-_INTS = (torch.int32, torch.int64)
+_INTS = {torch.int32: 0, torch.int64: 1}
 
 PerRow = Union[float, torch.Tensor, None]
 
 
-def _per_row(name: str, value: PerRow, neutral: float, B: int, dev, keep: list) -> tuple:
+def _per_row(name: str, value: PerRow, neutral: float, B: int, dev: int, keep: list) -> tuple:
     """(pointer, scalar) of a per-row fp32 value: a (B,) tensor, or a number
     for all rows."""
-    if value is None:
-        return 0, neutral
     if not isinstance(value, torch.Tensor):
         return 0, float(value)
-    assert value.shape == (B,) and value.device == dev and value.is_floating_point(), \
-        f"{name} must be a number or a float ({B},) tensor on {dev}"
+    assert value.shape == (B,) and value.get_device() == dev and value.is_floating_point(), \
+        f"{name} must be a number or a float ({B},) tensor on the logits' device"
     if value.dtype != torch.float32 or not value.is_contiguous():
         value = value.float().contiguous()
         keep.append(value)
     return value.data_ptr(), neutral
 
 
-def _row_ints(name: str, value: Optional[torch.Tensor], B: int, dev, keep: list) -> tuple:
+def _row_ints(name: str, value: torch.Tensor, B: int, dev: int, keep: list) -> tuple:
     """(pointer, is int64) of a (B,) integer tensor."""
-    if value is None:
-        return 0, 0
-    assert value.shape == (B,) and value.device == dev and value.dtype in _INTS, \
-        f"{name} must be an int32 or int64 ({B},) tensor on {dev}"
+    i64 = _INTS.get(value.dtype)
+    assert i64 is not None and value.shape == (B,) and value.get_device() == dev, \
+        f"{name} must be an int32 or int64 ({B},) tensor on the logits' device"
     if not value.is_contiguous():
         value = value.contiguous()
         keep.append(value)
-    return value.data_ptr(), int(value.dtype == torch.int64)
+    return value.data_ptr(), i64
 
 
-def _shared_rows(name: str, value: Optional[torch.Tensor], dtype: torch.dtype, B: int, width: int, dev,
+def _shared_rows(name: str, value: torch.Tensor, dtype: torch.dtype, B: int, width: int, dev: int,
                  keep: list) -> tuple:
     """(pointer, row stride) of a (width,) or (B, width) tensor."""
-    if value is None:
-        return 0, 0
-    assert value.device == dev and value.dim() in (1, 2) and value.shape[-1] >= width and \
-        (value.dim() == 1 or value.shape[0] in (1, B)), \
-        f"{name} must be ({width},) or ({B}, {width}) on {dev}, got {tuple(value.shape)} on {value.device}"
+    shape = value.shape
+    assert value.get_device() == dev and len(shape) in (1, 2) and shape[-1] >= width and \
+        (len(shape) == 1 or shape[0] == B or shape[0] == 1), \
+        f"{name} must be ({width},) or ({B}, {width}) on the logits' device, got {tuple(shape)}"
     if value.dtype != dtype or (value.stride(-1) != 1 and width > 1):
         value = value.to(dtype).contiguous()
         keep.append(value)
-    return value.data_ptr(), value.stride(0) if value.dim() == 2 and value.shape[0] > 1 else 0
+    return value.data_ptr(), value.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
 
 
 def _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
                  bias, allowed, keep: list) -> tuple:
     """Checked arguments that both entry points share: the packed fields up
     to ``allowed``, with the sampling ones open."""
-    assert logits.is_cuda and logits.dim() == 2, "logits must be a (B, V) CUDA tensor"
+    dev = logits.get_device() if logits.is_cuda else -1
+    assert dev >= 0 and logits.dim() == 2, "logits must be a (B, V) CUDA tensor"
     B, V = logits.shape
-    dev = logits.device
     code = _CODE.get(logits.dtype)
     assert code is not None, f"logits must be float32 or bfloat16 (got {logits.dtype})"
-    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+    if (logits.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("the logit operators have no gradient: call them under torch.no_grad() or detach")
-    if logits.stride(1) != 1 and V > 1:
-        logits = logits.contiguous()
-        keep.append(logits)
-    T = t_ptr = t_stride = t_i64 = 0
+    if logits.is_contiguous():
+        ld = V
+    else:
+        if logits.stride(1) != 1 and V > 1:
+            logits = logits.contiguous()
+            keep.append(logits)
+        ld = logits.stride(0)
+    T = t_ptr = t_stride = t_i64 = len_ptr = len_i64 = pro_ptr = pro_i64 = 0
     if tokens is not None:
-        assert tokens.dim() == 2 and tokens.shape[0] == B and tokens.device == dev and tokens.dtype in _INTS, \
-            f"tokens must be an int32 or int64 ({B}, T) tensor on {dev}"
-        T = tokens.shape[1]
-        if tokens.stride(1) != 1 and T > 1:
-            tokens = tokens.contiguous()
-            keep.append(tokens)
-        t_ptr, t_stride, t_i64 = tokens.data_ptr(), tokens.stride(0), int(tokens.dtype == torch.int64)
+        t_i64 = _INTS.get(tokens.dtype)
+        shape = tokens.shape
+        assert t_i64 is not None and len(shape) == 2 and shape[0] == B and tokens.get_device() == dev, \
+            f"tokens must be an int32 or int64 ({B}, T) tensor on the logits' device"
+        T = shape[1]
+        if tokens.is_contiguous():
+            t_stride = T
+        else:
+            if tokens.stride(1) != 1 and T > 1:
+                tokens = tokens.contiguous()
+                keep.append(tokens)
+            t_stride = tokens.stride(0)
+        t_ptr = tokens.data_ptr()
+        if lengths is not None:
+            len_ptr, len_i64 = _row_ints("lengths", lengths, B, dev, keep)
+        if prompt_lengths is not None:
+            pro_ptr, pro_i64 = _row_ints("prompt_lengths", prompt_lengths, B, dev, keep)
     else:
         assert lengths is None and prompt_lengths is None, "lengths and prompt_lengths go with tokens"
-    len_ptr, len_i64 = _row_ints("lengths", lengths, B, dev, keep)
-    pro_ptr, pro_i64 = _row_ints("prompt_lengths", prompt_lengths, B, dev, keep)
-    rep = _per_row("repetition_penalty", repetition_penalty, 1.0, B, dev, keep)
-    pres = _per_row("presence_penalty", presence_penalty, 0.0, B, dev, keep)
-    freq = _per_row("frequency_penalty", frequency_penalty, 0.0, B, dev, keep)
-    if not rep[0] and not rep[1] > 0:
-        raise ValueError(f"repetition_penalty must be above 0 (got {rep[1]})")
+    rep = pres = freq = mask_ptr = mask_stride = bias_ptr = bias_stride = 0
+    rep_value, pres_value, freq_value = 1.0, 0.0, 0.0
+    if repetition_penalty is not None:
+        rep, rep_value = _per_row("repetition_penalty", repetition_penalty, 1.0, B, dev, keep)
+        if not rep_value > 0:
+            raise ValueError(f"repetition_penalty must be above 0 (got {rep_value})")
+    if presence_penalty is not None:
+        pres, pres_value = _per_row("presence_penalty", presence_penalty, 0.0, B, dev, keep)
+    if frequency_penalty is not None:
+        freq, freq_value = _per_row("frequency_penalty", frequency_penalty, 0.0, B, dev, keep)
     if bias is not None:
         assert bias.is_floating_point(), "bias must be a float tensor"
-    bias_ptr, bias_stride = _shared_rows("bias", bias, torch.float32, B, V, dev, keep)
+        bias_ptr, bias_stride = _shared_rows("bias", bias, torch.float32, B, V, dev, keep)
     if allowed is not None:
         assert allowed.dtype == torch.int32, "allowed must hold the mask's bits in int32 words"
-    mask_ptr, mask_stride = _shared_rows("allowed", allowed, torch.int32, B, -(-V // 32), dev, keep)
-    head = (B, V, T, code, logits.data_ptr(), logits.stride(0), t_ptr, t_stride, len_ptr, pro_ptr, t_i64, len_i64,
-            pro_i64)
-    mid = (rep[0], pres[0], freq[0], rep[1], pres[1], freq[1])
-    return dev, head, mid, (bias_ptr, bias_stride, mask_ptr, mask_stride)
+        mask_ptr, mask_stride = _shared_rows("allowed", allowed, torch.int32, B, -(-V // 32), dev, keep)
+    return (dev, B, V,
+            (B, V, T, code, logits.data_ptr(), ld, t_ptr, t_stride, len_ptr, pro_ptr, t_i64, len_i64, pro_i64),
+            (rep, pres, freq, rep_value, pres_value, freq_value), (bias_ptr, bias_stride, mask_ptr, mask_stride))
 
 
 def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
@@ -137,23 +149,25 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             works in place.  A new tensor of the logits' type without it.
     """
     keep: list = []
-    dev, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
-                                        presence_penalty, frequency_penalty, bias, allowed, keep)
-    B, V = logits.shape
+    dev, B, V, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
+                                              presence_penalty, frequency_penalty, bias, allowed, keep)
+    out_ld = V
     if out is None:
-        out = logits.new_empty((B, V))
+        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
     else:
-        assert out.shape == logits.shape and out.device == dev and out.dtype in _CODE, \
-            f"out must be a float32 or bfloat16 {(B, V)} tensor on {dev}"
+        assert out.shape == logits.shape and out.device == logits.device and out.dtype in _CODE, \
+            f"out must be a float32 or bfloat16 {(B, V)} tensor on the logits' device"
         assert (V <= 1 or out.stride(1) == 1) and (B <= 1 or out.stride(0) >= V), \
             "out must have unit column stride and rows that do not overlap"
         if out is not logits and _overlap(out, logits):
             assert out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and \
                 out.stride() == logits.stride(), "out may be the logits themselves, not overlap them otherwise"
+        if B > 1:
+            out_ld = out.stride(0)
     if B == 0 or V == 0:
         return out
     nat.call("m3_process_logits", nat.LOGITS_ARGS.pack(
-        *head, 0, *mid, 0.0, *tail, out.data_ptr(), out.stride(0) if B > 1 else V, _CODE[out.dtype], 0, 0, 0, 0, 0, 0),
+        *head, 0, *mid, 0.0, *tail, out.data_ptr(), out_ld, _CODE[out.dtype], 0, 0, 0, 0, 0, 0),
         dev)
     return out
 
@@ -193,23 +207,26 @@ def next_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     masked is taken as the largest, with logprob NaN; a row with nothing
     allowed gives token 0 with logprob -inf."""
     keep: list = []
-    dev, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
-                                        presence_penalty, frequency_penalty, bias, allowed, keep)
-    B, V = logits.shape
+    dev, B, V, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
+                                              presence_penalty, frequency_penalty, bias, allowed, keep)
     assert V > 0, "next_tokens needs at least one logit a row"
-    sample = temperature is not None
-    temp = _per_row("temperature", temperature, 0.0, B, dev, keep)
+    sample = 0
+    temp, temp_value = 0, 0.0
     seed_ptr = pos_ptr = 0
-    if sample:
+    if temperature is not None:
+        sample = 1
+        temp, temp_value = _per_row("temperature", temperature, 0.0, B, dev, keep)
         assert seeds is not None, "a temperature needs seeds"
         assert seeds.dtype == torch.int64 and (positions is None or positions.dtype == torch.int64), \
             "seeds and positions must be int64"
         seed_ptr, _ = _row_ints("seeds", seeds, B, dev, keep)
-        pos_ptr, _ = _row_ints("positions", positions, B, dev, keep)
-    ids = logits.new_empty((B,), dtype=torch.int64)
-    logprobs = logits.new_empty((B,), dtype=torch.float32)
+        if positions is not None:
+            pos_ptr, _ = _row_ints("positions", positions, B, dev, keep)
+    device = logits.device
+    ids = torch.empty((B,), dtype=torch.int64, device=device)
+    logprobs = torch.empty((B,), dtype=torch.float32, device=device)
     if B > 0:
         nat.call("m3_next_tokens", nat.LOGITS_ARGS.pack(
-            *head, int(sample), *mid, temp[1], *tail, 0, 0, 0, 0, temp[0], seed_ptr, pos_ptr, ids.data_ptr(),
+            *head, sample, *mid, temp_value, *tail, 0, 0, 0, 0, temp, seed_ptr, pos_ptr, ids.data_ptr(),
             logprobs.data_ptr()), dev)
     return ids, logprobs
