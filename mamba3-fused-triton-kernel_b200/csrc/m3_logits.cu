@@ -196,31 +196,22 @@ struct Run {
 };
 
 __device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int bf16, int e, int n, int vec) {
-  if (bf16) {
-    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(row) + e;
-    if (vec && n >= kVec) {
-      uint32_t w[4];
+  if (!vec || n < kVec) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&v);
-      }
-      *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+    for (int i = 0; i < kVec; ++i)
+      if (i < n) st_any(row, e + i, z[i], bf16 ? M3_BF16 : M3_F32);
+  } else if (bf16) {
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (i < n) p[i] = __float2bfloat16_rn(z[i]);
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&v);
     }
+    *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(row) + e) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    float *p = static_cast<float *>(row) + e;
-    if (vec && n >= kVec) {
-      reinterpret_cast<float4 *>(p)[0] = make_float4(z[0], z[1], z[2], z[3]);
-      reinterpret_cast<float4 *>(p)[1] = make_float4(z[4], z[5], z[6], z[7]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (i < n) p[i] = z[i];
-    }
+    float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(row) + e);
+    p[0] = make_float4(z[0], z[1], z[2], z[3]);
+    p[1] = make_float4(z[4], z[5], z[6], z[7]);
   }
 }
 
@@ -236,22 +227,27 @@ struct Row {
   __device__ __forceinline__ uint32_t count(int o) const {
     return wide ? counts[o] : counts[o >> 1] >> ((o & 1) * 16) & 0xffffu;
   }
-  // the run of n logits at e, the window's o; ok: its bits of the mask
-  __device__ __forceinline__ void adjust(float (&z)[kVec], int e, int o, int n, uint32_t ok) const {
-    if (seen) {
-      const uint32_t hit = seen[o >> 5] >> (o & 31) & 0xffu;
-      if (hit) {
+  // which of the run at o have been seen
+  __device__ __forceinline__ uint32_t hits(int o) const { return seen ? seen[o >> 5] >> (o & 31) & 0xffu : 0u; }
+  __device__ __forceinline__ float penalized(float v, int o) const {
+    v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+    const uint32_t c = count(o);
+    return c ? __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres) : v;
+  }
+  __device__ __forceinline__ void penalize(float (&z)[kVec], int o, uint32_t hit) const {
+    while (hit) {
+      const int at = __ffs(hit) - 1;
+      hit &= hit - 1;
+      float v = z[0];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          if (!(hit >> i & 1u)) continue;
-          float v = z[i];
-          v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-          const uint32_t c = count(o + i);
-          if (c) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)c)), pres);
-          z[i] = v;
-        }
-      }
+      for (int i = 1; i < kVec; ++i) v = i == at ? z[i] : v;
+      v = penalized(v, o + at);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) z[i] = i == at ? v : z[i];
     }
+  }
+  // bias and mask of the run of n logits at e; ok: its bits of the mask
+  __device__ __forceinline__ void finish(float (&z)[kVec], int e, int n, uint32_t ok) const {
     if (bias) {
       if (vec_bias && n >= kVec) {
         const float4 b0 = reinterpret_cast<const float4 *>(bias + e)[0];
@@ -275,7 +271,7 @@ struct Row {
 // Marks and counts the history's tokens in [w0, w0 + n); held: the first
 // kTokens of every thread, read already (-1: not in the vocabulary).
 __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int w0, int n,
-                                             const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
+                                                 const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
   const m3_logits_args &a = p.a;
   const int tid = threadIdx.x, nt = blockDim.x;
   const int64_t at = (int64_t)row * a.tokens_stride;
@@ -294,18 +290,18 @@ __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int
     else
       atomicAdd(&counts[o >> 1], 1u << ((o & 1) * 16));
   };
-  const int rest = kTokens * nt + tid;  // the thread's first token that is not held
   for (int i = tid; i < p.window / 32; i += nt) seen[i] = 0u;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k)
     if (tid + k * nt < len) mark(held[k] - w0);
-  for (int i = rest; i < len; i += nt) mark(load_int(a.tokens, at + i, a.tokens_i64) - w0);
+  for (int64_t i = tid + (int64_t)kTokens * nt; i < len; i += nt)
+    mark(load_int(a.tokens, at + i, a.tokens_i64) - w0);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k)
     if (tid + k * nt < len && tid + k * nt >= prompt) count(held[k] - w0);
-  for (int i = rest; i < len; i += nt)
+  for (int64_t i = tid + (int64_t)kTokens * nt; i < len; i += nt)
     if (i >= prompt) count(load_int(a.tokens, at + i, a.tokens_i64) - w0);
   __syncthreads();
 }
@@ -377,7 +373,8 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
     uint32_t ok = 0u;
     fetch(q, ok, w0 + o, wn - o);
     q.get(z);
-    r.adjust(z, w0 + o, o, wn - o, ok);
+    r.penalize(z, o, r.hits(o));
+    r.finish(z, w0 + o, wn - o, ok);
   };
 
   const int step = nt * kVec;
@@ -399,6 +396,13 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
     if (MODE == kDraw && tid == 0) reached = -CUDART_INF_F;
     float most = -CUDART_INF_F, second = -CUDART_INF_F;  // highest bounds of its runs
     int most_at = -1;
+    // of bounds past fp32's range too the last run is kept
+    auto raise = [&](float b, int o) {
+      if (b >= most)
+        second = most, most = b, most_at = o;
+      else
+        second = fmaxf(second, b);
+    };
     for (int o0 = tid * kVec; o0 < wn; o0 += kRuns * step) {
 #pragma unroll
       for (int u = 0; u < kRuns; ++u) {
@@ -408,7 +412,8 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
         next[u].get(z);
         const uint32_t ok = next_ok[u];
         fetch(next[u], next_ok[u], w0 + o + kRuns * step, n - kRuns * step);
-        r.adjust(z, w0 + o, o, n, ok);
+        r.penalize(z, o, r.hits(o));
+        r.finish(z, w0 + o, n, ok);
         if (MODE == kProcess) {
           store_run(z, static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
                     a.out_dtype == M3_BF16, w0 + o, n, p.vec_out);
@@ -432,11 +437,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
 #pragma unroll
             for (int i = 0; i < 4; ++i) b = fmaxf(b, bound(z[4 * h + i], pick(w, i)));
           }
-          // of bounds past fp32's range too the last run is kept
-          if (b >= most)
-            second = most, most = b, most_at = o;
-          else
-            second = fmaxf(second, b);
+          raise(b, o);
         }
       }
     }
@@ -615,13 +616,14 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   p.window = p.history ? min(p.slice, p.wide ? kWindow / 2 : kWindow) : p.slice;
   const int64_t grid = (int64_t)a.B * p.slices;
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+  const int threads = min(kLogitThreads, ((p.slice + kVec - 1) / kVec + 31) / 32 * 32);
   auto kern = logits_kernel<T, MODE>;
   const size_t smem = p.history ? (size_t)p.window / 8 + (size_t)p.window * (p.wide ? 4 : 2) : 0;
   static LaunchCache cache;
   if (cudaError_t e = ensure_smem_optin(cache, kern, kWindow / 8 + kWindow * 2); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)min(kLogitThreads, ((p.slice + kVec - 1) / kVec + 31) / 32 * 32));
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

@@ -132,37 +132,53 @@ struct W4X<float> {
   }
 };
 
-// One block's codes and scales of a warp, in registers.
+// A lane's two rows of a row block: where their codes, scales and zeros are.
+struct W4Rows {
+  const uint4 *codes;
+  int64_t s[2], z[2];
+  __device__ __forceinline__ void set(const W4Params &p, int rb, int lane) {
+    codes = p.codes + (int64_t)rb * p.tiles * 64 + lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t n = min(rb * 16 + h * 8 + (lane >> 2), p.N - 1);  // rows past the last reach no output
+      s[h] = n * p.s_ld, z[h] = n * p.z_ld;
+    }
+  }
+};
+
+// One block's codes, scales and zeros of a lane as they lie in memory:
+// nothing is computed from them before they are used, so that a load waits
+// for none before it.
 template <int GPT>
 struct W4Stage {
   uint4 c[2];
-  float s[2][GPT];
-  uint32_t z[2][GPT];
-};
-
-// Block (rb, kt) of the weight: rows 16 rb + g and + 8.
-template <int GPT>
-__device__ __forceinline__ void w4_load(W4Stage<GPT> &st, const W4Params &p, int rb, int kt, int lane) {
-  const uint4 *c = p.codes + ((int64_t)rb * p.tiles + kt) * 64 + lane;
+  uint32_t s[2][GPT], z[2][GPT];
+  __device__ __forceinline__ void load(const W4Params &p, const W4Rows &r, int kt) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    st.c[h] = w4_codes(c + h * 32);
-    const int64_t n = min(rb * 16 + h * 8 + (lane >> 2), p.N - 1);  // rows past the last reach no output
+    for (int h = 0; h < 2; ++h) c[h] = w4_codes(r.codes + (int64_t)kt * 64 + h * 32);
 #pragma unroll
     for (int j = 0; j < GPT; ++j) {
       const int gi = min(kt * GPT + j, p.groups - 1);  // a group wholly past K has a sum of 0
-      st.s[h][j] = p.s_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.scales)[n * p.s_ld + gi])
-                            : static_cast<const float *>(p.scales)[n * p.s_ld + gi];
-      const uint32_t z = p.zeros ? (uint32_t)p.zeros[n * p.z_ld + gi] : 8u;
-      st.z[h][j] = 0x43004300u + z + (z << 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h][j] = p.s_bf16 ? (uint32_t) static_cast<const uint16_t *>(p.scales)[r.s[h] + gi]
+                           : static_cast<const uint32_t *>(p.scales)[r.s[h] + gi];
+        if (p.zeros) z[h][j] = p.zeros[r.z[h] + gi];
+      }
     }
   }
-}
+  __device__ __forceinline__ float scale(const W4Params &p, int h, int j) const {
+    return __uint_as_float(p.s_bf16 ? s[h][j] << 16 : s[h][j]);
+  }
+  __device__ __forceinline__ uint32_t bias(const W4Params &p, int h, int j) const {  // (128 + z, 128 + z)
+    return 0x43004300u + (p.zeros ? z[h][j] * 0x10001u : 0x80008u);
+  }
+};
 
 // tot += the block's products with MT 8-row batch tiles; get(o, j, b) gives
 // the terms of x for run j of the tile and batch tile b.
 template <int MT, int GPT, int TERMS, typename Get>
-__device__ __forceinline__ void w4_block(float (&tot)[MT][4], const W4Stage<GPT> &st, Get get) {
+__device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4], const W4Stage<GPT> &st, Get get) {
   constexpr int PER = 4 / GPT;  // 32-column runs of a group
   float d[MT][4];
 #pragma unroll
@@ -177,9 +193,10 @@ __device__ __forceinline__ void w4_block(float (&tot)[MT][4], const W4Stage<GPT>
     uint32_t w[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const uint32_t zz = st.bias(p, h, gj);
       const uint32_t word = j == 0 ? st.c[h].x : j == 1 ? st.c[h].y : j == 2 ? st.c[h].z : st.c[h].w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[h][i] = w4_pair(word, i, st.z[h][gj]);
+      for (int i = 0; i < 4; ++i) w[h][i] = w4_pair(word, i, zz);
     }
 #pragma unroll
     for (int b = 0; b < MT; ++b) {
@@ -192,10 +209,11 @@ __device__ __forceinline__ void w4_block(float (&tot)[MT][4], const W4Stage<GPT>
       }
     }
     if (j % PER == PER - 1) {
+      const float s[2] = {st.scale(p, 0, gj), st.scale(p, 1, gj)};
 #pragma unroll
       for (int b = 0; b < MT; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tot[b][e] = fmaf(d[b][e], st.s[e >> 1][gj], tot[b][e]);
+        for (int e = 0; e < 4; ++e) tot[b][e] = fmaf(d[b][e], s[e >> 1], tot[b][e]);
     }
   }
 }
@@ -254,10 +272,15 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
   pdl_trigger();
 
   int lrb = rb0, lk = wk;  // the next block to load
+  W4Rows rows_of;
+  rows_of.set(p, min(lrb, p.blocks - 1), lane);
   auto load = [&](W4Stage<GPT> &st) {
-    if (lrb < p.blocks && lk < p.tiles) w4_load(st, p, lrb, lk, lane);
+    if (lrb < p.blocks && lk < p.tiles) st.load(p, rows_of, lk);
     lk += p.wk;
-    if (lk >= spt * p.wk) lk = wk, lrb += rstep;
+    if (lk >= spt * p.wk) {
+      lk = wk, lrb += rstep;
+      rows_of.set(p, min(lrb, p.blocks - 1), lane);
+    }
   };
   W4Stage<GPT> st[kW4Depth];
 #pragma unroll
@@ -292,7 +315,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
         }
         if (kt < p.tiles) {
           const uint4 *xs = w4_smem + (int64_t)kt * 4 * MT * TERMS * 32 + lane;
-          w4_block<MT, GPT, TERMS>(tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
+          w4_block<MT, GPT, TERMS>(p, tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
 #pragma unroll
             for (int q = 0; q < TERMS; ++q) o[q] = xs[((j * MT + b) * TERMS + q) * 32];
           });
@@ -342,10 +365,12 @@ __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mt
   pdl_wait();
   pdl_trigger();
   W4Stage<GPT> cur, nxt;
-  if (wk < p.tiles) w4_load(cur, p, rb, wk, lane);
+  W4Rows rows_of;
+  rows_of.set(p, rb, lane);
+  if (wk < p.tiles) cur.load(p, rows_of, wk);
   for (int kt = wk; kt < p.tiles; kt += WK) {
-    if (kt + WK < p.tiles) w4_load(nxt, p, rb, kt + WK, lane);
-    w4_block<MT, GPT, X::kTerms>(tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
+    if (kt + WK < p.tiles) nxt.load(p, rows_of, kt + WK);
+    w4_block<MT, GPT, X::kTerms>(p, tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
       const int m = m0 + b * 8 + g;
       X xv;
       if (m < p.M)

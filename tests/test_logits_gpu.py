@@ -360,3 +360,17 @@ def test_refusals():
                 z.flatten()[1:].as_strided((2, 99), (99, 1)), torch.empty(2, 100)):
         with pytest.raises(AssertionError):
             process_logits(z[:, :out.shape[1]] if out.shape[1] == 99 else z, out=out)
+
+
+@pytest.mark.parametrize("V", [600, 60000])
+@pytest.mark.parametrize("T", [3000, 16384, 16385, 70000])
+def test_long_histories(V, T):
+    """Past what a thread holds, past 16-bit counters, in several windows."""
+    a = case(2, V, T, torch.float32, seed=T, mask="row")
+    a["lengths"][:] = T
+    a["prompt_lengths"][:] = torch.tensor([0, T // 2], device="cuda")
+    a["tokens"][0, : T - 100] = V - 1
+    check_process(a)
+    check_process(dict(a, logits=a["logits"].bfloat16()))
+    check_next(a)
+    check_next(a, 0.9, torch.tensor([5, 6], device="cuda"))
