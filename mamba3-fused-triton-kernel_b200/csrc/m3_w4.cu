@@ -132,16 +132,28 @@ struct W4X<float> {
   }
 };
 
-// A lane's two rows of a row block: where their codes, scales and zeros are.
-struct W4Rows {
-  const uint4 *codes;
-  int64_t s[2], z[2];
-  __device__ __forceinline__ void set(const W4Params &p, int rb, int lane) {
-    codes = p.codes + (int64_t)rb * p.tiles * 64 + lane;
+// Where a lane's next block is: its codes, and the scales and zeros of its
+// two rows (g and g + 8 of the row block).
+template <int GPT, bool ZEROS>
+struct W4At {
+  const uint4 *c;
+  const char *s[2];
+  const uint8_t *z[2];
+  __device__ __forceinline__ void set(const W4Params &p, int rb, int kt, int lane) {
+    c = p.codes + ((int64_t)rb * p.tiles + kt) * 64 + lane;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t n = min(rb * 16 + h * 8 + (lane >> 2), p.N - 1);  // rows past the last reach no output
-      s[h] = n * p.s_ld, z[h] = n * p.z_ld;
+      s[h] = static_cast<const char *>(p.scales) + ((n * p.s_ld + kt * GPT) << (p.s_bf16 ? 1 : 2));
+      if (ZEROS) z[h] = p.zeros + n * p.z_ld + kt * GPT;
+    }
+  }
+  __device__ __forceinline__ void advance(const W4Params &p, int tiles) {
+    c += tiles * 64;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] += (tiles * GPT) << (p.s_bf16 ? 1 : 2);
+      if (ZEROS) z[h] += tiles * GPT;
     }
   }
 };
@@ -149,38 +161,41 @@ struct W4Rows {
 // One block's codes, scales and zeros of a lane as they lie in memory:
 // nothing is computed from them before they are used, so that a load waits
 // for none before it.
-template <int GPT>
+template <int GPT, bool ZEROS>
 struct W4Stage {
   uint4 c[2];
   uint32_t s[2][GPT], z[2][GPT];
-  __device__ __forceinline__ void load(const W4Params &p, const W4Rows &r, int kt) {
+  __device__ __forceinline__ void load(const W4Params &p, const W4At<GPT, ZEROS> &at, int kt) {
+    c[0] = w4_codes(at.c), c[1] = w4_codes(at.c + 32);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) c[h] = w4_codes(r.codes + (int64_t)kt * 64 + h * 32);
-#pragma unroll
-    for (int j = 0; j < GPT; ++j) {
-      const int gi = min(kt * GPT + j, p.groups - 1);  // a group wholly past K has a sum of 0
+    for (int j = 0; j < GPT; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s[h][j] = p.s_bf16 ? (uint32_t) static_cast<const uint16_t *>(p.scales)[r.s[h] + gi]
-                           : static_cast<const uint32_t *>(p.scales)[r.s[h] + gi];
-        if (p.zeros) z[h][j] = p.zeros[r.z[h] + gi];
+        const bool in = GPT == 1 || kt * GPT + j < p.groups;  // a group wholly past K has a sum of 0
+        s[h][j] = !in ? 0u
+                      : p.s_bf16 ? (uint32_t) reinterpret_cast<const uint16_t *>(at.s[h])[j]
+                                 : reinterpret_cast<const uint32_t *>(at.s[h])[j];
+        if (ZEROS) z[h][j] = in ? at.z[h][j] : 0u;
       }
-    }
   }
   __device__ __forceinline__ float scale(const W4Params &p, int h, int j) const {
     return __uint_as_float(p.s_bf16 ? s[h][j] << 16 : s[h][j]);
   }
-  __device__ __forceinline__ uint32_t bias(const W4Params &p, int h, int j) const {  // (128 + z, 128 + z)
-    return 0x43004300u + (p.zeros ? z[h][j] * 0x10001u : 0x80008u);
+  __device__ __forceinline__ uint32_t bias(int h, int j) const {  // (128 + z, 128 + z)
+    return ZEROS ? 0x43004300u + z[h][j] * 0x10001u : 0x43084308u;
   }
 };
 
 // tot += the block's products with MT 8-row batch tiles; get(o, j, b) gives
-// the terms of x for run j of the tile and batch tile b.
-template <int MT, int GPT, int TERMS, typename Get>
-__device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4], const W4Stage<GPT> &st, Get get) {
+// the terms of x for run j of the tile and batch tile b.  A run's two MMAs go
+// to sums of their own where one batch tile would leave the chain of
+// dependent MMAs bare.
+template <int MT, int GPT, bool ZEROS, int TERMS, typename Get>
+__device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4], const W4Stage<GPT, ZEROS> &st,
+                                         Get get) {
   constexpr int PER = 4 / GPT;  // 32-column runs of a group
-  float d[MT][4];
+  constexpr int CHAINS = MT == 1 ? 2 : 1;
+  float d[MT][CHAINS][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int gj = j / PER;
@@ -188,12 +203,14 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4],
 #pragma unroll
       for (int b = 0; b < MT; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[b][e] = 0.f;
+        for (int c = 0; c < CHAINS; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[b][c][e] = 0.f;
     }
     uint32_t w[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t zz = st.bias(p, h, gj);
+      const uint32_t zz = st.bias(h, gj);
       const uint32_t word = j == 0 ? st.c[h].x : j == 1 ? st.c[h].y : j == 2 ? st.c[h].z : st.c[h].w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[h][i] = w4_pair(word, i, zz);
@@ -204,8 +221,8 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4],
       get(o, j, b);
 #pragma unroll
       for (int q = TERMS - 1; q >= 0; --q) {  // small terms first
-        w4_mma(d[b], w[0][0], w[1][0], w[0][1], w[1][1], o[q].x, o[q].y);
-        w4_mma(d[b], w[0][2], w[1][2], w[0][3], w[1][3], o[q].z, o[q].w);
+        w4_mma(d[b][0], w[0][0], w[1][0], w[0][1], w[1][1], o[q].x, o[q].y);
+        w4_mma(d[b][CHAINS - 1], w[0][2], w[1][2], w[0][3], w[1][3], o[q].z, o[q].w);
       }
     }
     if (j % PER == PER - 1) {
@@ -213,7 +230,8 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4],
 #pragma unroll
       for (int b = 0; b < MT; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tot[b][e] = fmaf(d[b][e], s[e >> 1], tot[b][e]);
+        for (int e = 0; e < 4; ++e)
+          tot[b][e] = fmaf(CHAINS == 2 ? d[b][0][e] + d[b][CHAINS - 1][e] : d[b][0][e], s[e >> 1], tot[b][e]);
     }
   }
 }
@@ -225,9 +243,15 @@ __device__ __forceinline__ void w4_store(const W4Params &p, int m, int n, float 
     static_cast<float *>(p.y)[(int64_t)m * p.ldy + n] = s;
 }
 
-constexpr int kW4Warps = 16;
-constexpr int kW4Depth = 3;                   // blocks a warp has in flight
-constexpr int kW4SmemBudget = 200 * 1024;     // x and the partial sums
+constexpr int kW4SmemBudget = 200 * 1024;  // x and the partial sums
+
+// Warps of a CTA: with one batch tile the registers allow twice as many,
+// which the chain unpack - MMA - scale of a block needs.
+template <int MT>
+constexpr int w4_warps() { return MT == 1 ? 32 : 16; }
+// Blocks a warp has in flight, as registers allow: 64 KB an SM or more.
+template <int MT>
+constexpr int w4_depth() { return MT == 1 ? 2 : 3; }
 
 // Partial sums of a warp: 16 rows by MT * 8 batch rows, padded against bank conflicts
 constexpr int kW4RowLd = 17;
@@ -242,14 +266,14 @@ int64_t w4_stream_smem(int tiles, int wk, int wn) {
 
 // The decode batches' kernel: persistent CTAs that hold all of x in shared
 // memory, in fragment order, and stream blocks of codes through registers,
-// kW4Depth ahead.  A CTA's p.wk x p.wn warps are p.wn groups; a group takes
-// row blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of one, and
+// a few ahead.  A CTA's p.wk x p.wn warps are p.wn groups; a group takes row
+// blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of one, and
 // their sums are added in warp order through shared memory (two buffers and
 // one barrier of the group per row block).
-template <typename XT, int MT, int GPT>
-__global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Params p) {
+template <typename XT, int MT, int GPT, bool ZEROS>
+__global__ void __launch_bounds__(w4_warps<MT>() * 32, 1) w4_stream_kernel(const W4Params p) {
   using X = W4X<XT>;
-  constexpr int TERMS = X::kTerms, RED = w4_red_floats<MT>();
+  constexpr int TERMS = X::kTerms, RED = w4_red_floats<MT>(), DEPTH = w4_depth<MT>();
   extern __shared__ __align__(16) uint4 w4_smem[];
   const int pieces = p.tiles * 4 * MT * 32;
   float *red = reinterpret_cast<float *>(w4_smem + (int64_t)pieces * TERMS);
@@ -257,13 +281,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
   const int wk = warp % p.wk, wn = warp / p.wk;
   const int m0 = (int)(blockIdx.x % p.mtiles) * MT * 8, rows = min(p.M - m0, MT * 8);
   const int rb0 = (int)(blockIdx.x / p.mtiles) * p.wn + wn, rstep = (int)(gridDim.x / p.mtiles) * p.wn;
-  const int spt = (p.tiles + p.wk - 1) / p.wk;  // steps of a row block
-  const int rounds = rb0 < p.blocks ? (p.blocks - rb0 + rstep - 1) / rstep : 0;
-  const int total = rounds * spt;
+  const int steps = wk < p.tiles ? (p.tiles - wk + p.wk - 1) / p.wk : 0;  // of this warp in a row block
 
   // the first blocks into L2 while the preceding kernel runs
-  if (total > 0 && wk == 0 && lane == 0) {
-    const uint32_t bytes = (uint32_t)min(p.tiles, kW4Depth * p.wk) * 1024u;
+  if (rb0 < p.blocks && wk == 0 && lane == 0) {
+    const uint32_t bytes = (uint32_t)min(p.tiles, DEPTH * p.wk) * 1024u;
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.codes + (int64_t)rb0 * p.tiles * 64),
                  "r"(bytes)
                  : "memory");
@@ -272,19 +294,24 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
   pdl_trigger();
 
   int lrb = rb0, lk = wk;  // the next block to load
-  W4Rows rows_of;
-  rows_of.set(p, min(lrb, p.blocks - 1), lane);
-  auto load = [&](W4Stage<GPT> &st) {
-    if (lrb < p.blocks && lk < p.tiles) st.load(p, rows_of, lk);
+  W4At<GPT, ZEROS> at;
+  if (steps > 0) at.set(p, min(lrb, p.blocks - 1), lk, lane);
+  auto load = [&](W4Stage<GPT, ZEROS> &st) {
+    if (lrb >= p.blocks) return;
+    st.load(p, at, lk);
     lk += p.wk;
-    if (lk >= spt * p.wk) {
+    if (lk < p.tiles) {
+      at.advance(p, p.wk);
+    } else {
       lk = wk, lrb += rstep;
-      rows_of.set(p, min(lrb, p.blocks - 1), lane);
+      if (lrb < p.blocks) at.set(p, lrb, lk, lane);
     }
   };
-  W4Stage<GPT> st[kW4Depth];
+  W4Stage<GPT, ZEROS> st[DEPTH];
+  if (steps > 0) {
 #pragma unroll
-  for (int u = 0; u < kW4Depth; ++u) load(st[u]);
+    for (int u = 0; u < DEPTH; ++u) load(st[u]);
+  }
 
   for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
     const int l = i & 31, b = (i >> 5) % MT, kj = (i >> 5) / MT;
@@ -302,43 +329,55 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
   __syncthreads();
 
   float tot[MT][4];
-  int step = 0, kt = wk, rb = rb0, parity = 0;
-  for (int it = 0; it < total; it += kW4Depth) {
+  // the row block is done: its sums, added over the group's warps
+  auto finish = [&](int rb, int parity) {
+    // element e of a tile: weight row g + 8 (e / 2), batch row 2 t + e % 2
+    float *group = red + (parity * p.wn + wn) * p.wk * RED;
+    float *mine = group + wk * RED;
 #pragma unroll
-    for (int u = 0; u < kW4Depth; ++u) {
-      if (it + u < total) {
-        if (step == 0) {
+    for (int b = 0; b < MT; ++b)
 #pragma unroll
-          for (int b = 0; b < MT; ++b)
+      for (int e = 0; e < 4; ++e)
+        mine[(b * 8 + 2 * (lane & 3) + (e & 1)) * kW4RowLd + (e >> 1) * 8 + (lane >> 2)] = tot[b][e];
+    if (p.wk > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(wn), "r"(p.wk * 32) : "memory");
+    else
+      __syncwarp();
+    for (int i = wk * 32 + lane; i < rows * 16; i += p.wk * 32) {
+      const int r = i & 15, m = i >> 4, n = rb * 16 + r;
+      float s = group[m * kW4RowLd + r];
+      for (int k = 1; k < p.wk; ++k) s += group[k * RED + m * kW4RowLd + r];
+      if (n < p.N) w4_store(p, m0 + m, n, s);
+    }
+  };
+  auto clear = [&] {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
-        }
-        if (kt < p.tiles) {
-          const uint4 *xs = w4_smem + (int64_t)kt * 4 * MT * TERMS * 32 + lane;
-          w4_block<MT, GPT, TERMS>(p, tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
+    for (int b = 0; b < MT; ++b)
 #pragma unroll
-            for (int q = 0; q < TERMS; ++q) o[q] = xs[((j * MT + b) * TERMS + q) * 32];
-          });
-        }
+      for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
+  };
+  const int xstep = 4 * MT * TERMS * 32;  // pieces of a tile
+  int rb = rb0, left = steps, parity = 0;
+  const uint4 *xs = w4_smem + (int64_t)wk * xstep + lane;
+  clear();
+  if (steps == 0) {  // more warps than tiles: zeros to the sums
+    for (; rb < p.blocks; rb += rstep, parity ^= 1) finish(rb, parity);
+    return;
+  }
+  while (rb < p.blocks) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      if (rb < p.blocks) {
+        w4_block<MT, GPT, ZEROS, TERMS>(p, tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
+#pragma unroll
+          for (int q = 0; q < TERMS; ++q) o[q] = xs[((j * MT + b) * TERMS + q) * 32];
+        });
         load(st[u]);
-        kt += p.wk;
-        if (++step == spt) {
-          // element e of a tile: weight row g + 8 (e / 2), batch row 2 t + e % 2
-          float *group = red + (parity * p.wn + wn) * p.wk * RED;
-          float *mine = group + wk * RED;
-#pragma unroll
-          for (int b = 0; b < MT; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mine[(b * 8 + 2 * (lane & 3) + (e & 1)) * kW4RowLd + (e >> 1) * 8 + (lane >> 2)] = tot[b][e];
-          asm volatile("bar.sync %0, %1;" ::"r"(wn + 1 <= 15 ? wn + 1 : 0), "r"(p.wk * 32) : "memory");
-          for (int i = wk * 32 + lane; i < rows * 16; i += p.wk * 32) {
-            const int r = i & 15, m = i >> 4, n = rb * 16 + r;
-            float s = group[m * kW4RowLd + r];
-            for (int k = 1; k < p.wk; ++k) s += group[k * RED + m * kW4RowLd + r];
-            if (n < p.N) w4_store(p, m0 + m, n, s);
-          }
-          parity ^= 1, step = 0, kt = wk, rb += rstep;
+        xs += p.wk * xstep;
+        if (--left == 0) {
+          finish(rb, parity);
+          clear();
+          parity ^= 1, left = steps, rb += rstep, xs = w4_smem + (int64_t)wk * xstep + lane;
         }
       }
     }
@@ -347,7 +386,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) w4_stream_kernel(const W4Par
 
 // Any batch and any K: the same blocks, x read where it is.  A CTA is 8 warps,
 // 2 along K by 4 row blocks that share x through L1.
-template <typename XT, int MT, int GPT>
+template <typename XT, int MT, int GPT, bool ZEROS>
 __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mtiles) {
   using X = W4X<XT>;
   constexpr int WK = 2, WN = 4, COLS = MT * 8;
@@ -364,13 +403,14 @@ __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mt
     for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
   pdl_wait();
   pdl_trigger();
-  W4Stage<GPT> cur, nxt;
-  W4Rows rows_of;
-  rows_of.set(p, rb, lane);
-  if (wk < p.tiles) cur.load(p, rows_of, wk);
+  W4Stage<GPT, ZEROS> cur, nxt;
+  W4At<GPT, ZEROS> at;
+  at.set(p, rb, wk, lane);
+  if (wk < p.tiles) cur.load(p, at, wk);
   for (int kt = wk; kt < p.tiles; kt += WK) {
-    if (kt + WK < p.tiles) nxt.load(p, rows_of, kt + WK);
-    w4_block<MT, GPT, X::kTerms>(p, tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
+    at.advance(p, WK);
+    if (kt + WK < p.tiles) nxt.load(p, at, kt + WK);
+    w4_block<MT, GPT, ZEROS, X::kTerms>(p, tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
       const int m = m0 + b * 8 + g;
       X xv;
       if (m < p.M)
@@ -393,33 +433,33 @@ __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mt
   }
 }
 
-template <typename XT, int MT, int GPT>
+template <typename XT, int MT, int GPT, bool ZEROS>
 cudaError_t launch_w4_direct(const W4Params &p, cudaStream_t stream) {
   const int mtiles = (p.M + MT * 8 - 1) / (MT * 8);
   const int64_t grid = (int64_t)((p.blocks + 3) / 4) * mtiles;
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(w4_direct_kernel<XT, MT, GPT>, dim3((unsigned)grid), dim3(256), 0, stream, p, mtiles);
+  return launch_pdl(w4_direct_kernel<XT, MT, GPT, ZEROS>, dim3((unsigned)grid), dim3(256), 0, stream, p, mtiles);
 }
 
 // Warps along K: the split with the fewest steps of the busiest warp (fewest
 // warps a row block on ties: less to add up), then as many row blocks per CTA
 // as keep every SM busy.
-template <typename XT, int MT, int GPT>
+template <typename XT, int MT, int GPT, bool ZEROS>
 cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
-  constexpr int TERMS = W4X<XT>::kTerms;
+  constexpr int TERMS = W4X<XT>::kTerms, WARPS = w4_warps<MT>();
   p.mtiles = (p.M + MT * 8 - 1) / (MT * 8);
   const int sms = max(1, sm_count_current() / p.mtiles);  // of a batch tile
   int64_t best = INT64_MAX;
-  for (int wk = 1; wk <= kW4Warps; wk *= 2) {
-    const int64_t streams = (int64_t)sms * (kW4Warps / wk);
+  for (int wk = WARPS / 16; wk <= WARPS; wk *= 2) {  // at most 16 groups: a barrier each
+    const int64_t streams = (int64_t)sms * (WARPS / wk);
     const int64_t steps = (p.blocks + streams - 1) / streams * ((p.tiles + wk - 1) / wk);
     if (steps < best) best = steps, p.wk = wk;
   }
-  p.wn = min(kW4Warps / p.wk, (p.blocks + sms - 1) / sms);
+  p.wn = min(WARPS / p.wk, (p.blocks + sms - 1) / sms);
   const int64_t smem = w4_stream_smem<MT, TERMS>(p.tiles, p.wk, p.wn);
   *taken = smem <= kW4SmemBudget;
   if (!*taken) return cudaSuccess;
-  auto kern = w4_stream_kernel<XT, MT, GPT>;
+  auto kern = w4_stream_kernel<XT, MT, GPT, ZEROS>;
   static LaunchCache cache;
   if (cudaError_t e = ensure_smem_optin(cache, kern, kW4SmemBudget); e != cudaSuccess) return e;
   const int64_t grid = (int64_t)min(sms, (p.blocks + p.wn - 1) / p.wn) * p.mtiles;
@@ -427,22 +467,27 @@ cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
   return launch_pdl(kern, dim3((unsigned)grid), dim3(p.wk * p.wn * 32), (size_t)smem, stream, p);
 }
 
-template <typename XT, int GPT>
+template <typename XT, int GPT, bool ZEROS>
 cudaError_t launch_w4_x(const W4Params &p, cudaStream_t stream) {
   bool taken = false;
   cudaError_t e = cudaSuccess;
   // the largest batch tile whose x fits in shared memory
-  if (p.M > 16) e = launch_w4_stream<XT, 4, GPT>(p, stream, &taken);
-  if (!taken && e == cudaSuccess && p.M > 8) e = launch_w4_stream<XT, 2, GPT>(p, stream, &taken);
-  if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 1, GPT>(p, stream, &taken);
+  if (p.M > 16) e = launch_w4_stream<XT, 4, GPT, ZEROS>(p, stream, &taken);
+  if (!taken && e == cudaSuccess && p.M > 8) e = launch_w4_stream<XT, 2, GPT, ZEROS>(p, stream, &taken);
+  if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 1, GPT, ZEROS>(p, stream, &taken);
   if (taken || e != cudaSuccess) return e;
-  return p.M <= 8 ? launch_w4_direct<XT, 1, GPT>(p, stream) : launch_w4_direct<XT, 4, GPT>(p, stream);
+  return p.M <= 8 ? launch_w4_direct<XT, 1, GPT, ZEROS>(p, stream) : launch_w4_direct<XT, 4, GPT, ZEROS>(p, stream);
+}
+
+template <typename XT, int GPT>
+cudaError_t launch_w4_z(const W4Params &p, cudaStream_t stream) {
+  return p.zeros ? launch_w4_x<XT, GPT, true>(p, stream) : launch_w4_x<XT, GPT, false>(p, stream);
 }
 
 template <typename XT>
 cudaError_t launch_w4_g(const W4Params &p, int group, cudaStream_t stream) {
-  return group == 128 ? launch_w4_x<XT, 1>(p, stream)
-                      : group == 64 ? launch_w4_x<XT, 2>(p, stream) : launch_w4_x<XT, 4>(p, stream);
+  return group == 128 ? launch_w4_z<XT, 1>(p, stream)
+                      : group == 64 ? launch_w4_z<XT, 2>(p, stream) : launch_w4_z<XT, 4>(p, stream);
 }
 
 }  // namespace
