@@ -6,7 +6,10 @@ Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` (one process per file,
 in parallel) and links ``lib/libmamba3_b200.so`` with the CUDA runtime linked
 statically, so the library only needs the driver at run time.  Objects go to
 ``_build/`` next to this file.  A file is rebuilt when it or any header under
-``csrc/`` / the repository ``include/`` is newer than its object.
+``csrc/`` / the repository ``include/`` is newer than its object.  Also builds
+``lib/m3_host.so`` from ``csrc/m3_host.cpp`` (a Python module on PyTorch's C++
+interface, no CUDA code): the host-side fast path of the language-model
+operators.
 """
 
 from __future__ import annotations
@@ -18,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -26,6 +30,8 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(HERE, "_build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmamba3_b200.so")
+HOST_SRC = os.path.join(CSRC, "m3_host.cpp")
+HOST_LIB = os.path.join(LIBDIR, "m3_host.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3",
@@ -83,7 +89,30 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int = 0) -> st
         os.replace(tmp, LIB)
     if ptxas_verbose:
         sys.stderr.write("".join(logs))
+    build_host(nvcc, force)
     return LIB
+
+
+def build_host(nvcc: str, force: bool = False) -> None:
+    """``lib/m3_host.so``, with the C++ compiler and the headers of the
+    PyTorch that this interpreter imports."""
+    newest = max(os.path.getmtime(HOST_SRC), *(os.path.getmtime(h) for h in glob.glob(os.path.join(INCLUDE, "*.h"))))
+    if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= newest:
+        return
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include"), INCLUDE]
+    libs = os.path.join(base, "lib")
+    tmp = HOST_LIB + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + i for i in inc), HOST_SRC,
+           "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST_LIB)
 
 
 def main():

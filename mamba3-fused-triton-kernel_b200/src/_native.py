@@ -16,6 +16,7 @@ src/kernels/siso_decode.py:157-159) and an unsupported MIMO rank becomes
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 import threading
@@ -203,6 +204,34 @@ def require_cuda_available(what: str = "the CUDA decode backend") -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+HOST_PATH = os.path.join(os.path.dirname(LIB_PATH), "m3_host.so")
+_host = None
+
+
+def _no_host(*args):
+    """Stands for an entry of the host module where that is not built."""
+    return None
+
+
+def host_entry(name: str):
+    """The host module's function ``name`` (csrc/m3_host.cpp): called with an
+    operator's positional arguments it returns the result, or None for a call
+    it leaves to the Python path, which does the same work with a few more
+    microseconds of host time."""
+    global _host
+    if _host is None:
+        if not os.path.exists(HOST_PATH):
+            return _no_host
+        lib = load()
+        spec = importlib.util.spec_from_file_location("m3_host", HOST_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, f), c_void_p).value
+                      for f in ("m3_linear_w4", "m3_process_logits", "m3_next_tokens")))
+        _host = module
+    return getattr(_host, name)
 
 
 def call(name: str, args: bytes, index: int) -> None:

@@ -175,6 +175,8 @@ class W4Projection:
         self.key = (w.data_ptr(), w._version, w.dtype)
 
 
+_host = None  # the host module's linear_w4, once looked up
+
 _CODE = {torch.float32: nat.M3_F32, torch.bfloat16: nat.M3_BF16}
 
 
@@ -187,6 +189,13 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     type by default).  Written for the batches of a decode step, right for
     any M.  The codes' products with x must stay within fp32's range before
     the scale.  Inference only: x with a gradient is refused."""
+    global _host
+    if out_dtype is None:
+        if _host is None:
+            _host = nat.host_entry("linear_w4")
+        y = _host(x, codes, scales, zeros, group_size)
+        if y is not None:
+            return y
     if group_size not in GROUP_SIZES:
         _check_group(group_size)
     dev = x.get_device() if x.is_cuda else -1

@@ -29,6 +29,8 @@ _INTS = {torch.int32: 0, torch.int64: 1}
 
 PerRow = Union[float, torch.Tensor, None]
 
+_host_process = _host_next = None  # the host module's functions, once looked up
+
 
 def _per_row(name: str, value: PerRow, neutral: float, B: int, dev: int, keep: list) -> tuple:
     """(pointer, scalar) of a per-row fp32 value: a (B,) tensor, or a number
@@ -148,6 +150,14 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     out     (B, V) float32 or bfloat16, unit column stride; ``logits`` itself
             works in place.  A new tensor of the logits' type without it.
     """
+    global _host_process
+    if out is None:
+        if _host_process is None:
+            _host_process = nat.host_entry("process_logits")
+        y = _host_process(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
+                          frequency_penalty, bias, allowed)
+        if y is not None:
+            return y
     keep: list = []
     dev, B, V, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
                                               presence_penalty, frequency_penalty, bias, allowed, keep)
@@ -206,6 +216,13 @@ def next_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     row was drawn from (greedy rows: at temperature 1).  A NaN that is not
     masked is taken as the largest, with logprob NaN; a row with nothing
     allowed gives token 0 with logprob -inf."""
+    global _host_next
+    if _host_next is None:
+        _host_next = nat.host_entry("next_tokens")
+    both = _host_next(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
+                      frequency_penalty, bias, allowed, temperature, seeds, positions)
+    if both is not None:
+        return both
     keep: list = []
     dev, B, V, head, mid, tail = _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty,
                                               presence_penalty, frequency_penalty, bias, allowed, keep)

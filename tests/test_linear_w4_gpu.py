@@ -3,6 +3,8 @@ stand for."""
 
 from __future__ import annotations
 
+import importlib
+
 import pytest
 import torch
 
@@ -191,3 +193,24 @@ def test_refusals():
         linear_w4(x.requires_grad_(), w.codes, w.scales, **ok)
     with torch.no_grad():
         linear_w4(x, w.codes, w.scales, **ok)
+
+
+def test_host_module_and_python_path_agree(monkeypatch):
+    """The host module serves the ordinary call and leaves the others."""
+    from src import _native as nat
+    mod = importlib.import_module("src.kernels.linear_w4")
+    host = nat.host_entry("linear_w4")
+    assert host is not nat._no_host, "lib/m3_host.so is not built"
+    w = make(100, 300, 64, True)
+    x = torch.randn(5, 300, device="cuda")
+    y = host(x, w.codes, w.scales, w.zeros, 64)
+    assert y is not None and torch.equal(host(x, w.codes, w.scales, None, 64),
+                                         linear_w4(x, w.codes, w.scales, group_size=64))
+    for args in ((x.t().contiguous().t(), w.codes, w.scales, w.zeros, 64), (x, w.codes, w.scales, w.zeros, 128),
+                 (x.half(), w.codes, w.scales, w.zeros, 64), (x.cpu(), w.codes, w.scales, w.zeros, 64),
+                 (x, w.codes[:1], w.scales, w.zeros, 64), (x, w.codes, w.scales, w.zeros.int(), 64),
+                 (x[:0], w.codes, w.scales, w.zeros, 64), (x.clone().requires_grad_(), w.codes, w.scales, w.zeros, 64),
+                 (x, w.codes, None, w.zeros, 64), (x, w.codes, w.scales, w.zeros)):
+        assert host(*args) is None
+    monkeypatch.setattr(mod, "_host", nat._no_host)
+    assert torch.equal(linear_w4(x, w.codes, w.scales, w.zeros, group_size=64), y)

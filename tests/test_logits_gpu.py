@@ -3,6 +3,7 @@ bits for the sums and word by word for the random numbers."""
 
 from __future__ import annotations
 
+import importlib
 import math
 
 import numpy as np
@@ -374,3 +375,43 @@ def test_long_histories(V, T):
     check_process(dict(a, logits=a["logits"].bfloat16()))
     check_next(a)
     check_next(a, 0.9, torch.tensor([5, 6], device="cuda"))
+
+
+@pytest.mark.parametrize("python_path", [False, True])
+def test_host_module_and_python_path_agree(python_path, monkeypatch):
+    """The host module serves the ordinary calls; both ways are the formula."""
+    from src import _native as nat
+    mod = importlib.import_module("src.kernels.logits")
+    assert nat.host_entry("next_tokens") is not nat._no_host, "lib/m3_host.so is not built"
+    if python_path:
+        monkeypatch.setattr(mod, "_host_process", nat._no_host)
+        monkeypatch.setattr(mod, "_host_next", nat._no_host)
+    seeds, pos = torch.arange(4, device="cuda"), torch.arange(4, device="cuda") + 2 ** 35
+    for bias, mask in ((None, None), ("row", "shared"), ("shared", "row")):
+        a = case(4, 1000, 60, torch.float32, seed=11, bias=bias, mask=mask)
+        a["logits"] = a["logits"][:, :991]
+        a["tokens"] = a["tokens"].clamp(max=990)
+        if bias:
+            a["bias"] = a["bias"][..., :991]
+        check_process(a)
+        check_next(a)
+        check_next(a, 0.8, seeds, pos)
+        check_next(dict(a, repetition_penalty=1.25, presence_penalty=0.5, frequency_penalty=None), 0.8, seeds)
+        b = dict(a, lengths=a["lengths"].int(), prompt_lengths=None, tokens=a["tokens"].int())
+        check_process(b)
+
+
+def test_host_module_leaves_what_it_does_not_take():
+    from src import _native as nat
+    f = nat.host_entry("process_logits")
+    z, hist = torch.zeros(2, 100, device="cuda"), torch.zeros(2, 5, dtype=torch.long, device="cuda")
+    none = [None] * 8
+    assert f(z, *none) is not None
+    for args in ((z.half(), *none), (z[0], *none), (z.t().contiguous().t(), *none), (z[:0], *none), (z.cpu(), *none),
+                 (z.clone().requires_grad_(), *none), (z, hist[:1], *none[1:]), (z, hist.float(), *none[1:]),
+                 (z, None, hist[:, 0].contiguous(), *none[2:]), (z, hist, None, None, 0.0, *none[4:]),
+                 (z, hist, None, None, torch.ones(3, device="cuda"), *none[4:]), (z, *none[:6], torch.zeros(99, device="cuda"), None),
+                 (z, *none[:7], torch.zeros(3, dtype=torch.int32, device="cuda")), (z, *none[:7])):
+        assert f(*args) is None
+    g = nat.host_entry("next_tokens")
+    assert g(z, *none, 1.0, None, None) is None and g(z, *none, 1.0, torch.zeros(2, dtype=torch.int32, device="cuda"), None) is None
