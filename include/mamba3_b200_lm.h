@@ -37,6 +37,7 @@ extern "C" {
  *   zeros   (N, ceil(K / group)) bytes 0..15, row stride zero_stride, or NULL
  *   y       (M, N)  y_dtype (f32 / bf16), row stride ldy >= N, unit column stride
  *   group   32, 64 or 128
+ * Codes, scales and zeros take less than 4 GB each (M3_ERR_SHAPE).
  * Products are exact (a bf16 x times a small integer; an fp32 x is taken as
  * three bf16 terms), sums are fp32, scaled once per group and added in a
  * fixed order: the same call gives the same bits.  The sum of a group before

@@ -47,6 +47,13 @@ int m3_linear_w4(const m3_w4_args *a, m3_stream_t stream) {
   if (a->M < 0 || a->N <= 0 || a->K <= 0 || a->ldx < 0 || a->ldy < a->N) return M3_ERR_SHAPE;
   const int64_t groups = ((int64_t)a->K + a->group - 1) / a->group;
   if (a->scale_stride < groups || (a->zeros && a->zero_stride < groups)) return M3_ERR_SHAPE;
+  // the kernels' 32-bit byte offsets into codes, scales and zeros
+  const int64_t rows = ((int64_t)a->N + M3_W4_ROWS - 1) / M3_W4_ROWS;
+  const int64_t tiles = ((int64_t)a->K + M3_W4_TILE - 1) / M3_W4_TILE;
+  const int64_t most = (int64_t)1 << 32;
+  if (rows * tiles > most / 1024 || (a->N - 1) > (most / 4 - groups) / a->scale_stride ||
+      (a->zeros && (a->N - 1) > (most - groups) / a->zero_stride))
+    return M3_ERR_SHAPE;
   if (!aligned(a->codes, 16)) return M3_ERR_ALIGN;
   if (!dtype_aligned(a->x, a->x_dtype) || !dtype_aligned(a->scales, a->s_dtype) || !dtype_aligned(a->y, a->y_dtype))
     return M3_ERR_ALIGN;

@@ -35,7 +35,7 @@ __device__ __forceinline__ void w4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 
 // 16 bytes of codes, read once: past L1.  Volatile, so that it stays behind
 // the wait for the preceding kernel.
-__device__ __forceinline__ uint4 w4_codes(const uint4 *p) {
+__device__ __forceinline__ uint4 w4_codes(const char *p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
@@ -43,70 +43,92 @@ __device__ __forceinline__ uint4 w4_codes(const uint4 *p) {
   return v;
 }
 
-// Where a lane's next block is: its codes, and the scales and zeros of its
-// two rows (g and g + 8 of the row block).
-template <int GPT, bool ZEROS>
+// 16 bytes global -> shared, or 16 zero bytes
+__device__ __forceinline__ void w4_copy16(void *dst, const void *src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(real ? 16 : 0)
+               : "memory");
+}
+
+// Where a lane's next blocks are: the codes of NT row blocks (one tile each),
+// and the scales and zeros of its two rows (g and g + 8) of each.  32-bit byte
+// offsets: the launcher takes no weight past them.
+template <int NT, int GPT, bool ZEROS>
 struct W4At {
-  const uint4 *c;
-  const char *s[2];
-  const uint8_t *z[2];
+  uint32_t c[NT], s[NT][2], z[NT][2];
   __device__ __forceinline__ void set(const W4Params &p, int rb, int kt, int lane) {
-    c = p.codes + ((int64_t)rb * p.tiles + kt) * 64 + lane;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t n = min(rb * 16 + h * 8 + (lane >> 2), p.N - 1);  // rows past the last reach no output
-      s[h] = static_cast<const char *>(p.scales) + ((n * p.s_ld + kt * GPT) << (p.s_bf16 ? 1 : 2));
-      if (ZEROS) z[h] = p.zeros + n * p.z_ld + kt * GPT;
+    for (int a = 0; a < NT; ++a) {
+      const int block = min(rb * NT + a, p.blocks - 1);  // past the last: reaches no output
+      c[a] = ((uint32_t)block * p.tiles + kt) * 1024u + lane * 16u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t n = min(block * 16 + h * 8 + (lane >> 2), p.N - 1);
+        s[a][h] = (n * (uint32_t)p.s_ld + kt * GPT) << (p.s_bf16 ? 1 : 2);
+        if (ZEROS) z[a][h] = n * (uint32_t)p.z_ld + kt * GPT;
+      }
     }
   }
   __device__ __forceinline__ void advance(const W4Params &p, int tiles) {
-    c += tiles * 64;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] += (tiles * GPT) << (p.s_bf16 ? 1 : 2);
-      if (ZEROS) z[h] += tiles * GPT;
+    for (int a = 0; a < NT; ++a) {
+      c[a] += tiles * 1024u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[a][h] += (uint32_t)(tiles * GPT) << (p.s_bf16 ? 1 : 2);
+        if (ZEROS) z[a][h] += tiles * GPT;
+      }
     }
   }
 };
 
-// One block's codes, scales and zeros of a lane as they lie in memory:
+// The blocks' codes, scales and zeros of a lane as they lie in memory:
 // nothing is computed from them before they are used, so that a load waits
 // for none before it.
-template <int GPT, bool ZEROS>
+template <int NT, int GPT, bool ZEROS>
 struct W4Stage {
-  uint4 c[2];
-  uint32_t s[2][GPT], z[2][GPT];
-  __device__ __forceinline__ void load(const W4Params &p, const W4At<GPT, ZEROS> &at, int kt) {
-    c[0] = w4_codes(at.c), c[1] = w4_codes(at.c + 32);
+  uint4 c[NT][2];
+  uint32_t s[NT][2][GPT], z[NT][2][GPT];
+  __device__ __forceinline__ void load(const W4Params &p, const W4At<NT, GPT, ZEROS> &at, int kt) {
+    const char *codes = reinterpret_cast<const char *>(p.codes);
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+      c[a][0] = w4_codes(codes + at.c[a]);
+      c[a][1] = w4_codes(codes + at.c[a] + 512);
+    }
 #pragma unroll
     for (int j = 0; j < GPT; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool in = GPT == 1 || kt * GPT + j < p.groups;  // a group wholly past K has a sum of 0
-        s[h][j] = !in ? 0u
-                      : p.s_bf16 ? (uint32_t) reinterpret_cast<const uint16_t *>(at.s[h])[j]
-                                 : reinterpret_cast<const uint32_t *>(at.s[h])[j];
-        if (ZEROS) z[h][j] = in ? at.z[h][j] : 0u;
-      }
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool in = GPT == 1 || kt * GPT + j < p.groups;  // a group wholly past K has a sum of 0
+          const char *sp = static_cast<const char *>(p.scales) + at.s[a][h];
+          s[a][h][j] = !in ? 0u
+                           : p.s_bf16 ? (uint32_t) reinterpret_cast<const uint16_t *>(sp)[j]
+                                      : reinterpret_cast<const uint32_t *>(sp)[j];
+          if (ZEROS) z[a][h][j] = in ? p.zeros[at.z[a][h] + j] : 0u;
+        }
   }
-  __device__ __forceinline__ float scale(const W4Params &p, int h, int j) const {
-    return __uint_as_float(p.s_bf16 ? s[h][j] << 16 : s[h][j]);
+  __device__ __forceinline__ float scale(const W4Params &p, int a, int h, int j) const {
+    return __uint_as_float(p.s_bf16 ? s[a][h][j] << 16 : s[a][h][j]);
   }
-  __device__ __forceinline__ uint32_t bias(int h, int j) const {  // (128 + z, 128 + z)
-    return ZEROS ? 0x43004300u + z[h][j] * 0x10001u : 0x43084308u;
+  __device__ __forceinline__ uint32_t bias(int a, int h, int j) const {  // (128 + z, 128 + z)
+    return ZEROS ? 0x43004300u + z[a][h][j] * 0x10001u : 0x43084308u;
   }
 };
 
-// tot += the block's products with MT 8-row batch tiles; get(o, j, b) gives
-// the terms of x for run j of the tile and batch tile b.  A run's two MMAs go
-// to sums of their own where one batch tile would leave the chain of
-// dependent MMAs bare.
-template <int MT, int GPT, bool ZEROS, int TERMS, typename Get>
-__device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4], const W4Stage<GPT, ZEROS> &st,
-                                         Get get) {
+// tot += the products of NT row blocks with MT 8-row batch tiles; get(o, j, b)
+// gives the terms of x for run j of the tile and batch tile b, which the row
+// blocks share.  A run's two MMAs go to sums of their own where one tile
+// would leave the chain of dependent MMAs bare.
+template <int MT, int NT, int GPT, bool ZEROS, int TERMS, typename Get>
+__device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][NT][4],
+                                         const W4Stage<NT, GPT, ZEROS> &st, Get get) {
   constexpr int PER = 4 / GPT;  // 32-column runs of a group
-  constexpr int CHAINS = MT == 1 ? 2 : 1;
-  float d[MT][CHAINS][4];
+  constexpr int CHAINS = MT * NT == 1 ? 2 : 1;
+  float d[MT][NT][CHAINS][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int gj = j / PER;
@@ -114,70 +136,86 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][4],
 #pragma unroll
       for (int b = 0; b < MT; ++b)
 #pragma unroll
-        for (int c = 0; c < CHAINS; ++c)
+        for (int a = 0; a < NT; ++a)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[b][c][e] = 0.f;
+          for (int c = 0; c < CHAINS; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[b][a][c][e] = 0.f;
     }
-    uint32_t w[2][4];
+    uint32_t w[NT][2][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t zz = st.bias(h, gj);
-      const uint32_t word = j == 0 ? st.c[h].x : j == 1 ? st.c[h].y : j == 2 ? st.c[h].z : st.c[h].w;
+    for (int a = 0; a < NT; ++a)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[h][i] = w4_pair(word, i, zz);
-    }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t zz = st.bias(a, h, gj);
+        const uint4 c = st.c[a][h];
+        const uint32_t word = j == 0 ? c.x : j == 1 ? c.y : j == 2 ? c.z : c.w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[a][h][i] = w4_pair(word, i, zz, p.mask, p.magic);
+      }
 #pragma unroll
     for (int b = 0; b < MT; ++b) {
       uint4 o[TERMS];
       get(o, j, b);
 #pragma unroll
       for (int q = TERMS - 1; q >= 0; --q) {  // small terms first
-        w4_mma(d[b][0], w[0][0], w[1][0], w[0][1], w[1][1], o[q].x, o[q].y);
-        w4_mma(d[b][CHAINS - 1], w[0][2], w[1][2], w[0][3], w[1][3], o[q].z, o[q].w);
+#pragma unroll
+        for (int a = 0; a < NT; ++a) w4_mma(d[b][a][0], w[a][0][0], w[a][1][0], w[a][0][1], w[a][1][1], o[q].x, o[q].y);
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+          w4_mma(d[b][a][CHAINS - 1], w[a][0][2], w[a][1][2], w[a][0][3], w[a][1][3], o[q].z, o[q].w);
       }
     }
     if (j % PER == PER - 1) {
-      const float s[2] = {st.scale(p, 0, gj), st.scale(p, 1, gj)};
 #pragma unroll
-      for (int b = 0; b < MT; ++b)
+      for (int a = 0; a < NT; ++a) {
+        const float s[2] = {st.scale(p, a, 0, gj), st.scale(p, a, 1, gj)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          tot[b][e] = fmaf(CHAINS == 2 ? d[b][0][e] + d[b][CHAINS - 1][e] : d[b][0][e], s[e >> 1], tot[b][e]);
+        for (int b = 0; b < MT; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            tot[b][a][e] = fmaf(CHAINS == 2 ? d[b][a][0][e] + d[b][a][CHAINS - 1][e] : d[b][a][0][e], s[e >> 1],
+                                tot[b][a][e]);
+      }
     }
   }
 }
 
-constexpr int kW4SmemBudget = 200 * 1024;  // x and the partial sums
+constexpr int kW4SmemBudget = 227 * 1024;  // x and the partial sums: all an SM gives a CTA
 
-// Warps of a CTA: with one batch tile the registers allow twice as many,
-// which the chain unpack - MMA - scale of a block needs.
-template <int MT>
-constexpr int w4_warps() { return MT == 1 ? 32 : 16; }
-// Blocks a warp has in flight, as registers allow: 64 KB an SM or more.
-template <int MT>
-constexpr int w4_depth() { return MT == 1 ? 2 : 3; }
-
-// Partial sums of a warp: 16 rows by MT * 8 batch rows, padded against bank conflicts
-constexpr int kW4RowLd = 17;
-template <int MT>
-constexpr int w4_red_floats() { return MT * 8 * kW4RowLd; }
+// The shape of a CTA by its batch tiles MT.  One tile: as many warps as the
+// SM takes, which the chain unpack - MMA - scale of a block needs.  More:
+// two row blocks a warp, which share the batch operand's loads from shared
+// memory (two loads of 512 bytes feed as many MMAs as the SM can issue in
+// their time only then), and the registers for them.
+// Finer groups hold more scales in flight: fewer warps, or one row block.
+template <int MT, int GPT>
+struct W4Shape {
+  static constexpr int kWarps = MT == 1 ? (GPT == 1 ? 32 : GPT == 2 ? 24 : 16) : MT == 2 ? 16 : 12;
+  static constexpr int NT = MT == 1 || GPT == 4 ? 1 : 2;
+  static constexpr int kDepth = 2;                         // blocks a warp has in flight: 48 KB an SM or more
+  static constexpr int kLd = NT * 16 + 1;                  // partial sums of a batch row, padded against conflicts
+  static constexpr int kRed = MT * 8 * kLd;                // partial sums of a warp
+  static constexpr int kBufs = MT == 4 ? 1 : 2;            // of them: a second one saves a barrier, x wants the room
+};
 
 // x as the MMAs take it: [tile][run j][batch tile][term][lane] pieces of 16 bytes
-template <int MT, int TERMS>
+template <int MT, int GPT, int TERMS>
 int64_t w4_stream_smem(int tiles, int wk, int wn) {
-  return (int64_t)tiles * 4 * MT * TERMS * 512 + (int64_t)2 * wk * wn * w4_red_floats<MT>() * 4;
+  return (int64_t)tiles * 4 * MT * TERMS * 512 + (int64_t)W4Shape<MT, GPT>::kBufs * wk * wn * W4Shape<MT, GPT>::kRed * 4;
 }
 
 // The decode batches' kernel: persistent CTAs that hold all of x in shared
 // memory, in fragment order, and stream blocks of codes through registers,
-// a few ahead.  A CTA's p.wk x p.wn warps are p.wn groups; a group takes row
-// blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of one, and
-// their sums are added in warp order through shared memory (two buffers and
-// one barrier of the group per row block).
+// a few ahead.  A CTA's p.wk x p.wn warps are p.wn groups; a group takes NT
+// row blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of them, and
+// their sums are added in warp order through shared memory, behind a barrier
+// of the group.
 template <typename XT, int MT, int GPT, bool ZEROS>
-__global__ void __launch_bounds__(w4_warps<MT>() * 32, 1) w4_stream_kernel(const W4Params p) {
+__global__ void __launch_bounds__(W4Shape<MT, GPT>::kWarps * 32, 1) w4_stream_kernel(const W4Params p) {
   using X = W4X<XT>;
-  constexpr int TERMS = X::kTerms, RED = w4_red_floats<MT>(), DEPTH = w4_depth<MT>();
+  using S = W4Shape<MT, GPT>;
+  constexpr int TERMS = X::kTerms, NT = S::NT, RED = S::kRed, DEPTH = S::kDepth, ROWS = NT * 16, LD = S::kLd;
   extern __shared__ __align__(16) uint4 w4_smem[];
   const int pieces = p.tiles * 4 * MT * 32;
   float *red = reinterpret_cast<float *>(w4_smem + (int64_t)pieces * TERMS);
@@ -185,94 +223,139 @@ __global__ void __launch_bounds__(w4_warps<MT>() * 32, 1) w4_stream_kernel(const
   const int wk = warp % p.wk, wn = warp / p.wk;
   const int m0 = (int)(blockIdx.x % p.mtiles) * MT * 8, rows = min(p.M - m0, MT * 8);
   const int rb0 = (int)(blockIdx.x / p.mtiles) * p.wn + wn, rstep = (int)(gridDim.x / p.mtiles) * p.wn;
+  const int rbs = (p.blocks + NT - 1) / NT;
   const int steps = wk < p.tiles ? (p.tiles - wk + p.wk - 1) / p.wk : 0;  // of this warp in a row block
 
   // the first blocks into L2 while the preceding kernel runs
-  if (rb0 < p.blocks && wk == 0 && lane == 0) {
+  if (rb0 < rbs && wk == 0 && lane < NT && rb0 * NT + lane < p.blocks) {
     const uint32_t bytes = (uint32_t)min(p.tiles, DEPTH * p.wk) * 1024u;
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.codes + (int64_t)rb0 * p.tiles * 64),
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.codes + (int64_t)(rb0 * NT + lane) * p.tiles * 64),
                  "r"(bytes)
                  : "memory");
   }
   pdl_wait();  // x is the preceding kernel's output, and the weight may be too
   pdl_trigger();
 
-  int lrb = rb0, lk = wk;  // the next block to load
-  W4At<GPT, ZEROS> at;
-  if (steps > 0) at.set(p, min(lrb, p.blocks - 1), lk, lane);
-  auto load = [&](W4Stage<GPT, ZEROS> &st) {
-    if (lrb >= p.blocks) return;
+  int lrb = rb0, lk = wk;  // the next blocks to load
+  W4At<NT, GPT, ZEROS> at;
+  if (steps > 0) at.set(p, min(lrb, rbs - 1), lk, lane);
+  auto load = [&](W4Stage<NT, GPT, ZEROS> &st) {
+    if (lrb >= rbs) return;
     st.load(p, at, lk);
     lk += p.wk;
     if (lk < p.tiles) {
       at.advance(p, p.wk);
     } else {
       lk = wk, lrb += rstep;
-      if (lrb < p.blocks) at.set(p, lrb, lk, lane);
+      if (lrb < rbs) at.set(p, lrb, lk, lane);
     }
   };
-  W4Stage<GPT, ZEROS> st[DEPTH];
+  W4Stage<NT, GPT, ZEROS> st[DEPTH];
   if (steps > 0) {
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) load(st[u]);
   }
 
-  for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+  // x into shared memory: a bf16 piece is copied as it is, all copies in
+  // flight; fp32 and odd pieces go through registers, a few at a time
+  auto stage = [&](int i) {  // row and column of piece i
     const int l = i & 31, b = (i >> 5) % MT, kj = (i >> 5) / MT;
-    const int m = b * 8 + (l >> 2);
-    X xv;
-    if (m < rows)
-      xv.load(p.x, (int64_t)(m0 + m) * p.ldx, kj * 32 + 8 * (l & 3), p.K, p.x_vec);
-    else
-      xv.zero();
-    uint4 o[TERMS];
-    xv.terms(o);
+    return make_int2(b * 8 + (l >> 2), kj * 32 + 8 * (l & 3));
+  };
+  if (TERMS == 1 && p.x_vec) {
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+      const int2 at = stage(i);
+      const bool real = at.x < rows && at.y + 8 <= p.K;
+      if (at.x < rows && at.y < p.K && !real) {
+        X xv;
+        uint4 o[TERMS];
+        xv.load(p.x, (int64_t)(m0 + at.x) * p.ldx, at.y, p.K, false);
+        xv.terms(o);
+        w4_smem[i] = o[0];
+      } else {
+        const XT *src = static_cast<const XT *>(p.x) + (real ? (int64_t)(m0 + at.x) * p.ldx + at.y : 0);
+        w4_copy16(w4_smem + i, src, real);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    constexpr int AHEAD = TERMS == 1 ? 4 : 2;
+    for (int i0 = threadIdx.x; i0 < pieces; i0 += AHEAD * blockDim.x) {
+      X xv[AHEAD];
 #pragma unroll
-    for (int q = 0; q < TERMS; ++q) w4_smem[((i >> 5) * TERMS + q) * 32 + l] = o[q];
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = i0 + u * blockDim.x;
+        const int2 at = stage(i);
+        if (i < pieces && at.x < rows)
+          xv[u].load(p.x, (int64_t)(m0 + at.x) * p.ldx, at.y, p.K, p.x_vec);
+        else
+          xv[u].zero();
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = i0 + u * blockDim.x;
+        uint4 o[TERMS];
+        xv[u].terms(o);
+        if (i < pieces) {
+#pragma unroll
+          for (int q = 0; q < TERMS; ++q) w4_smem[((i >> 5) * TERMS + q) * 32 + (i & 31)] = o[q];
+        }
+      }
+    }
   }
   __syncthreads();
 
-  float tot[MT][4];
-  // the row block is done: its sums, added over the group's warps
+  float tot[MT][NT][4];
+  // the row blocks are done: their sums, added over the group's warps
   auto finish = [&](int rb, int parity) {
     // element e of a tile: weight row g + 8 (e / 2), batch row 2 t + e % 2
-    float *group = red + (parity * p.wn + wn) * p.wk * RED;
+    float *group = red + ((S::kBufs == 2 ? parity * p.wn : 0) + wn) * p.wk * RED;
     float *mine = group + wk * RED;
 #pragma unroll
     for (int b = 0; b < MT; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        mine[(b * 8 + 2 * (lane & 3) + (e & 1)) * kW4RowLd + (e >> 1) * 8 + (lane >> 2)] = tot[b][e];
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mine[(b * 8 + 2 * (lane & 3) + (e & 1)) * LD + a * 16 + (e >> 1) * 8 + (lane >> 2)] = tot[b][a][e];
     if (p.wk > 1)
       asm volatile("bar.sync %0, %1;" ::"r"(wn), "r"(p.wk * 32) : "memory");
     else
       __syncwarp();
-    for (int i = wk * 32 + lane; i < rows * 16; i += p.wk * 32) {
-      const int r = i & 15, m = i >> 4, n = rb * 16 + r;
-      float s = group[m * kW4RowLd + r];
-      for (int k = 1; k < p.wk; ++k) s += group[k * RED + m * kW4RowLd + r];
+    for (int i = wk * 32 + lane; i < rows * ROWS; i += p.wk * 32) {
+      const int r = i % ROWS, m = i / ROWS, n = rb * ROWS + r;
+      float s = group[m * LD + r];
+      for (int k = 1; k < p.wk; ++k) s += group[k * RED + m * LD + r];
       if (n < p.N) w4_store(p, m0 + m, n, s);
+    }
+    if (S::kBufs == 1) {  // the sums have been read
+      if (p.wk > 1)
+        asm volatile("bar.sync %0, %1;" ::"r"(wn), "r"(p.wk * 32) : "memory");
+      else
+        __syncwarp();
     }
   };
   auto clear = [&] {
 #pragma unroll
     for (int b = 0; b < MT; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tot[b][a][e] = 0.f;
   };
   const int xstep = 4 * MT * TERMS * 32;  // pieces of a tile
   int rb = rb0, left = steps, parity = 0;
   const uint4 *xs = w4_smem + (int64_t)wk * xstep + lane;
   clear();
   if (steps == 0) {  // more warps than tiles: zeros to the sums
-    for (; rb < p.blocks; rb += rstep, parity ^= 1) finish(rb, parity);
+    for (; rb < rbs; rb += rstep, parity ^= 1) finish(rb, parity);
     return;
   }
-  while (rb < p.blocks) {
+  while (rb < rbs) {
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
-      if (rb < p.blocks) {
-        w4_block<MT, GPT, ZEROS, TERMS>(p, tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
+      if (rb < rbs) {
+        w4_block<MT, NT, GPT, ZEROS, TERMS>(p, tot, st[u], [&](uint4 (&o)[TERMS], int j, int b) {
 #pragma unroll
           for (int q = 0; q < TERMS; ++q) o[q] = xs[((j * MT + b) * TERMS + q) * 32];
         });
@@ -288,33 +371,34 @@ __global__ void __launch_bounds__(w4_warps<MT>() * 32, 1) w4_stream_kernel(const
   }
 }
 
-// Any batch and any K: the same blocks, x read where it is.  A CTA is 8 warps,
-// 2 along K by 4 row blocks that share x through L1.
+// Any batch and any K (a weight of less than 4 GB): the same blocks, x read
+// where it is.  A CTA is 8 warps, 2 along K by 4 row blocks that share x
+// through L1.
 template <typename XT, int MT, int GPT, bool ZEROS>
 __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mtiles) {
   using X = W4X<XT>;
-  constexpr int WK = 2, WN = 4, COLS = MT * 8;
-  __shared__ float red[WN][WK][w4_red_floats<MT>()];
+  constexpr int WK = 2, WN = 4, COLS = MT * 8, LD = 17;
+  __shared__ float red[WN][WK][COLS * LD];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int wk = warp % WK, wn = warp / WK;
   const int m0 = (int)(blockIdx.x % mtiles) * COLS;
   const int rb = min((int)(blockIdx.x / mtiles) * WN + wn, p.blocks - 1);  // past the last: computed, not stored
-  float tot[MT][4];
+  float tot[MT][1][4];
 #pragma unroll
   for (int b = 0; b < MT; ++b)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tot[b][e] = 0.f;
+    for (int e = 0; e < 4; ++e) tot[b][0][e] = 0.f;
   pdl_wait();
   pdl_trigger();
-  W4Stage<GPT, ZEROS> cur, nxt;
-  W4At<GPT, ZEROS> at;
+  W4Stage<1, GPT, ZEROS> cur, nxt;
+  W4At<1, GPT, ZEROS> at;
   at.set(p, rb, wk, lane);
   if (wk < p.tiles) cur.load(p, at, wk);
   for (int kt = wk; kt < p.tiles; kt += WK) {
     at.advance(p, WK);
     if (kt + WK < p.tiles) nxt.load(p, at, kt + WK);
-    w4_block<MT, GPT, ZEROS, X::kTerms>(p, tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
+    w4_block<MT, 1, GPT, ZEROS, X::kTerms>(p, tot, cur, [&](uint4 (&o)[X::kTerms], int j, int b) {
       const int m = m0 + b * 8 + g;
       X xv;
       if (m < p.M)
@@ -328,12 +412,12 @@ __global__ void __launch_bounds__(256) w4_direct_kernel(const W4Params p, int mt
 #pragma unroll
   for (int b = 0; b < MT; ++b)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[wn][wk][(b * 8 + 2 * t + (e & 1)) * kW4RowLd + (e >> 1) * 8 + g] = tot[b][e];
+    for (int e = 0; e < 4; ++e) red[wn][wk][(b * 8 + 2 * t + (e & 1)) * LD + (e >> 1) * 8 + g] = tot[b][0][e];
   __syncthreads();
   for (int i = threadIdx.x; i < COLS * WN * 16; i += 256) {
     const int r = i & 15, w = (i >> 4) % WN, c = i / (WN * 16);
     const int m = m0 + c, n = ((int)(blockIdx.x / mtiles) * WN + w) * 16 + r;
-    if (m < p.M && n < p.N) w4_store(p, m, n, red[w][0][c * kW4RowLd + r] + red[w][1][c * kW4RowLd + r]);
+    if (m < p.M && n < p.N) w4_store(p, m, n, red[w][0][c * LD + r] + red[w][1][c * LD + r]);
   }
 }
 
@@ -350,23 +434,25 @@ cudaError_t launch_w4_direct(const W4Params &p, cudaStream_t stream) {
 // as keep every SM busy.
 template <typename XT, int MT, int GPT, bool ZEROS>
 cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
-  constexpr int TERMS = W4X<XT>::kTerms, WARPS = w4_warps<MT>();
+  using S = W4Shape<MT, GPT>;
+  constexpr int TERMS = W4X<XT>::kTerms, WARPS = S::kWarps;
   p.mtiles = (p.M + MT * 8 - 1) / (MT * 8);
   const int sms = max(1, sm_count_current() / p.mtiles);  // of a batch tile
+  const int rbs = (p.blocks + S::NT - 1) / S::NT;
   int64_t best = INT64_MAX;
-  for (int wk = WARPS / 16; wk <= WARPS; wk *= 2) {  // at most 16 groups: a barrier each
+  for (int wk = (WARPS + 15) / 16; wk <= WARPS; wk *= 2) {  // at most 16 groups: a barrier each
     const int64_t streams = (int64_t)sms * (WARPS / wk);
-    const int64_t steps = (p.blocks + streams - 1) / streams * ((p.tiles + wk - 1) / wk);
+    const int64_t steps = (rbs + streams - 1) / streams * ((p.tiles + wk - 1) / wk);
     if (steps < best) best = steps, p.wk = wk;
   }
-  p.wn = min(WARPS / p.wk, (p.blocks + sms - 1) / sms);
-  const int64_t smem = w4_stream_smem<MT, TERMS>(p.tiles, p.wk, p.wn);
+  p.wn = min(WARPS / p.wk, (rbs + sms - 1) / sms);
+  const int64_t smem = w4_stream_smem<MT, GPT, TERMS>(p.tiles, p.wk, p.wn);
   *taken = smem <= kW4SmemBudget;
   if (!*taken) return cudaSuccess;
   auto kern = w4_stream_kernel<XT, MT, GPT, ZEROS>;
   static LaunchCache cache;
   if (cudaError_t e = ensure_smem_optin(cache, kern, kW4SmemBudget); e != cudaSuccess) return e;
-  const int64_t grid = (int64_t)min(sms, (p.blocks + p.wn - 1) / p.wn) * p.mtiles;
+  const int64_t grid = (int64_t)min(sms, (rbs + p.wn - 1) / p.wn) * p.mtiles;
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
   return launch_pdl(kern, dim3((unsigned)grid), dim3(p.wk * p.wn * 32), (size_t)smem, stream, p);
 }
@@ -405,6 +491,7 @@ cudaError_t launch_linear_w4(const m3_w4_args &a, cudaStream_t stream) {
   const int es = a.x_dtype == M3_BF16 ? 2 : 4;
   p.x_vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx * es % 16 == 0;
   p.codes = reinterpret_cast<const uint4 *>(a.codes);
+  p.mask = 0x000F000Fu, p.magic = 0x43004300u;
   p.scales = a.scales, p.s_ld = a.scale_stride, p.s_bf16 = a.s_dtype == M3_BF16;
   p.groups = (int)(((int64_t)a.K + a.group - 1) / a.group);
   p.zeros = a.zeros, p.z_ld = a.zero_stride;

@@ -17,6 +17,7 @@ struct W4Params {
   int64_t ldx;
   int x_vec;  // every row of x starts on 16 bytes
   const uint4 *codes;
+  uint32_t mask, magic;  // constants of w4_pair
   const void *scales;
   int64_t s_ld;
   int s_bf16, groups;
@@ -29,8 +30,11 @@ struct W4Params {
 
 // pair i of a word as bf16 (q - z), with zz = (128 + z, 128 + z): 128 + q is
 // the bf16 whose mantissa ends in q, and the difference is exact
-__device__ __forceinline__ uint32_t w4_pair(uint32_t w, int i, uint32_t zz) {
-  uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+// (mask 0x000F000F and magic 0x43004300 are kernel parameters: as immediates
+// the and and the or would be two instructions)
+__device__ __forceinline__ uint32_t w4_pair(uint32_t w, int i, uint32_t zz, uint32_t mask, uint32_t magic) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));  // (a & b) | c
   __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&v), *reinterpret_cast<__nv_bfloat162 *>(&zz));
   return *reinterpret_cast<uint32_t *>(&d);
 }
