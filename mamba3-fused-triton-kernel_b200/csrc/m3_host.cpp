@@ -52,7 +52,7 @@ PyObject *linear_w4(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const int dev = x.get_device(), xd = dtype_code(x.scalar_type()), sd = dtype_code(scales.scalar_type());
   const int64_t M = x.size(0), K = x.size(1), N = scales.size(0), groups = scales.size(1);
   if (xd < 0 || sd < 0 || M <= 0 || K <= 0 || N <= 0 || M > INT32_MAX || K > INT32_MAX || N > INT32_MAX ||
-      !x.is_contiguous() || (x.requires_grad() && at::GradMode::is_enabled()) ||
+      !x.is_contiguous() || ((x.requires_grad() || scales.requires_grad()) && at::GradMode::is_enabled()) ||
       codes.scalar_type() != at::kInt || !codes.is_contiguous() || codes.size(0) != (N + 15) / 16 ||
       codes.size(1) != (K + 127) / 128 || codes.size(2) != 16 || codes.size(3) != 16 ||
       groups != (K + group - 1) / group || !scales.is_contiguous() || !on(codes, dev) || !on(scales, dev) ||

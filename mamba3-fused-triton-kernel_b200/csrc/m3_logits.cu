@@ -42,8 +42,10 @@ namespace {
 constexpr int kVec = 8;       // consecutive logits of a thread
 constexpr int kRuns = 2;      // such runs a thread loads at a time
 constexpr int kTokens = 4;    // tokens of the history a thread holds
-constexpr int kLogitThreads = 512;
-constexpr int kLogitWarps = kLogitThreads / 32;
+// Threads of a CTA, two CTAs an SM: draws want the registers of fewer threads
+// (256 rows of bf16 44 against 50 us), the others the loads of more.
+template <int MODE>
+constexpr int logit_threads() { return MODE == 2 ? 384 : 512; }
 constexpr int kWindow = 51200;   // logits whose 16-bit counters a CTA holds: two CTAs per SM
 constexpr int kCountMax = 65535;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -98,9 +100,10 @@ struct RowNoise {
     uint4 c = make_uint4(i, c1, c2, 0u);
 #pragma unroll
     for (int r = 0; r < 7; ++r) {
-      const uint64_t a = (uint64_t)c.x * kM0, b = (uint64_t)c.z * kM1;
-      c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ (k0 + r * kW0), (uint32_t)b,
-                     (uint32_t)(a >> 32) ^ c.w ^ (k1 + r * kW1), (uint32_t)a);
+      uint32_t ah, al, bh, bl;
+      asm("{\n\t.reg .u64 t;\n\tmul.wide.u32 t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=r"(al), "=r"(ah) : "r"(c.x), "r"(kM0));
+      asm("{\n\t.reg .u64 t;\n\tmul.wide.u32 t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=r"(bl), "=r"(bh) : "r"(c.z), "r"(kM1));
+      c = make_uint4(bh ^ c.y ^ (k0 + r * kW0), bl, ah ^ c.w ^ (k1 + r * kW1), al);
     }
     return c;
   }
@@ -307,7 +310,8 @@ __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int
 }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const LogitsParams p) {
+  constexpr int kLogitWarps = logit_threads<MODE>() / 32;
   extern __shared__ __align__(16) uint32_t table[];  // bitmap and counters of a window
   __shared__ float warp_f[kLogitWarps], warp_b[kLogitWarps];
   __shared__ Drawn warp_d[kLogitWarps];
@@ -358,23 +362,26 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
     noise.k0 = (uint32_t)seed, noise.k1 = (uint32_t)(seed >> 32);
     noise.c1 = (uint32_t)pos, noise.c2 = (uint32_t)(pos >> 32);
   }
-  const float scale = fminf(kLog2e / temp, FLT_MAX);  // exponents are taken to base 2
+  // exponents are taken to base 2; kept finite and above 0, so that -infinity stays it
+  const float scale = fmaxf(fminf(kLog2e / temp, FLT_MAX), FLT_MIN);
   auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
   if (MODE != kProcess) __syncthreads();  // `first` stands
 
-  auto fetch = [&](Run<T> &q, uint32_t &ok, int e, int n) {
+  // a run and the mask's word it lies in, as they are in memory: nothing is
+  // computed from them here, so that the loads wait for none before them
+  auto fetch = [&](Run<T> &q, uint32_t &word, int e, int n) {
     if (n <= 0) return;
     q.load(logits, e, n, p.vec_in);
-    ok = allowed ? (uint32_t)allowed[e >> 5] >> (e & 31) & 0xffu : 0xffu;
+    word = allowed ? (uint32_t)allowed[e >> 5] : 0xffffffffu;
   };
   // the run at window offset o, adjusted (again, for a closer look)
   auto look_at = [&](float (&z)[kVec], int w0, int wn, int o) {
     Run<T> q;
-    uint32_t ok = 0u;
-    fetch(q, ok, w0 + o, wn - o);
+    uint32_t word = 0u;
+    fetch(q, word, w0 + o, wn - o);
     q.get(z);
     r.penalize(z, o, r.hits(o));
-    r.finish(z, w0 + o, wn - o, ok);
+    r.finish(z, w0 + o, wn - o, word >> (o & 31) & 0xffu);
   };
 
   const int step = nt * kVec;
@@ -384,9 +391,9 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
   for (int w0 = lo; w0 < hi; w0 += p.window) {
     const int wn = min(p.window, hi - w0);
     Run<T> next[kRuns];
-    uint32_t next_ok[kRuns];
+    uint32_t next_word[kRuns];
 #pragma unroll
-    for (int u = 0; u < kRuns; ++u) fetch(next[u], next_ok[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
+    for (int u = 0; u < kRuns; ++u) fetch(next[u], next_word[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
     if (r.seen) {
       if (w0 > lo) __syncthreads();  // the table has been read
       mark_history(p, row, len, prompt, w0, wn, held, table, table + p.window / 32);
@@ -410,8 +417,8 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
         if (n <= 0) continue;
         float z[kVec];
         next[u].get(z);
-        const uint32_t ok = next_ok[u];
-        fetch(next[u], next_ok[u], w0 + o + kRuns * step, n - kRuns * step);
+        const uint32_t ok = next_word[u] >> (o & 31) & 0xffu;
+        fetch(next[u], next_word[u], w0 + o + kRuns * step, n - kRuns * step);
         r.penalize(z, o, r.hits(o));
         r.finish(z, w0 + o, n, ok);
         if (MODE == kProcess) {
@@ -429,7 +436,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) logits_kernel(const LogitsPa
 #pragma unroll
         for (int i = 0; i < kVec; ++i) part[i & 1] += exp2_approx((z[i] - ref) * scale);
         mass += part[0] + part[1];
-        if (MODE == kDraw && drawn) {
+        if (MODE == kDraw && drawn && m > -CUDART_INF_F) {  // a run that the mask leaves empty draws nothing
           float b = -CUDART_INF_F;
 #pragma unroll
           for (int h = 0; h < kVec / 4; ++h) {
@@ -603,6 +610,7 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   p.vec_bias = a.bias && rows_on_16(a.bias, a.bias_stride, a.B, 4);
   // CTAs of a row: what fills two CTAs an SM, at least one run a thread each;
   // those that have to meet are a cluster, a power of two up to 8
+  constexpr int kLogitThreads = logit_threads<MODE>();
   const int fill = 2 * sm_count_current() / a.B;
   const int runs = (int)(((int64_t)a.V + kLogitThreads * kVec - 1) / (kLogitThreads * kVec));
   int want = max(1, min(fill, runs));

@@ -184,15 +184,15 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][NT]
 constexpr int kW4SmemBudget = 227 * 1024;  // x and the partial sums: all an SM gives a CTA
 
 // The shape of a CTA by its batch tiles MT.  One tile: as many warps as the
-// SM takes, which the chain unpack - MMA - scale of a block needs.  More:
-// two row blocks a warp, which share the batch operand's loads from shared
-// memory (two loads of 512 bytes feed as many MMAs as the SM can issue in
-// their time only then), and the registers for them.
-// Finer groups hold more scales in flight: fewer warps, or one row block.
+// SM takes, which the chain unpack - MMA - scale of a block needs.  Two: two
+// row blocks a warp, which share the batch operand's loads from shared memory
+// (50,280 x 2,560, 16 rows: 26.6 against 32.0 us with one).  Four: one row
+// block and 16 warps (64 rows of 9,440 x 2,048: 13.9 against 16.5 us with two
+// and 12).  Finer groups hold more scales in flight: fewer warps, one block.
 template <int MT, int GPT>
 struct W4Shape {
-  static constexpr int kWarps = MT == 1 ? (GPT == 1 ? 32 : GPT == 2 ? 24 : 16) : MT == 2 ? 16 : 12;
-  static constexpr int NT = MT == 1 || GPT == 4 ? 1 : 2;
+  static constexpr int kWarps = MT == 1 ? (GPT == 1 ? 32 : GPT == 2 ? 24 : 16) : 16;
+  static constexpr int NT = MT == 2 && GPT != 4 ? 2 : 1;
   static constexpr int kDepth = 2;                         // blocks a warp has in flight: 48 KB an SM or more
   static constexpr int kLd = NT * 16 + 1;                  // partial sums of a batch row, padded against conflicts
   static constexpr int kRed = MT * 8 * kLd;                // partial sums of a warp

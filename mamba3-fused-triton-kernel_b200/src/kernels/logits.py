@@ -148,8 +148,12 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     allowed (W,) or (B, W) int32, W at least ceil(V / 32): bit i % 32 of word
             i // 32 says whether token i may follow
     out     (B, V) float32 or bfloat16, unit column stride; ``logits`` itself
-            works in place.  A new tensor of the logits' type without it.
-    """
+            works in place.  It overlaps no other argument.  A new tensor of
+            the logits' type without it.
+
+    Penalties given as tensors are not looked at by the host: a repetition
+    penalty is above 0.  Inference only: logits or a bias with a gradient are
+    refused."""
     global _host_process
     if out is None:
         if _host_process is None:

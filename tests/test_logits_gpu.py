@@ -415,3 +415,12 @@ def test_host_module_leaves_what_it_does_not_take():
         assert f(*args) is None
     g = nat.host_entry("next_tokens")
     assert g(z, *none, 1.0, None, None) is None and g(z, *none, 1.0, torch.zeros(2, dtype=torch.int32, device="cuda"), None) is None
+
+
+def test_infinite_temperature_is_uniform():
+    z = torch.full((2000, 8), -INF, device="cuda")
+    z[:, :4] = torch.tensor([0.0, 5.0, -3.0, 100.0], device="cuda")
+    ids, lp = next_tokens(z, temperature=float("inf"), seeds=torch.arange(2000, device="cuda"))
+    count = torch.bincount(ids.cpu(), minlength=8)
+    assert not count[4:].any() and bool(((count[:4] - 500.0).abs() <= 5 * (2000 * 0.25 * 0.75) ** 0.5).all())
+    torch.testing.assert_close(lp, torch.full_like(lp, -math.log(4.0)))
