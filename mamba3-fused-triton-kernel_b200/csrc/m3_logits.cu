@@ -12,6 +12,14 @@
 //     tokens) beside it.  A counter is cleared by the token that marks it, so
 //     nothing of the vocabulary's size is swept but the bitmap, and a logit
 //     that was never seen, nearly every one, costs one bit.
+//   * Rows of an odd length start anywhere.  A row is therefore counted from
+//     the 16-byte boundary at or before its start: place q of a row is its
+//     logit q - shift, shift < 8, so that every run but the first and the
+//     last is one or two vector loads, in all rows (256 x 50,277 bf16 adjusted
+//     in 14 us, 41 element by element).  Draws count from the logit itself,
+//     whose index the generator's blocks go by, and load odd rows element by
+//     element.  Where every row starts on a boundary all that is left out
+//     (greedy, 256 x 50,280 bf16: 12 against 14 us).
 //   * Penalties, bias and mask are applied in fp32 operation by operation (no
 //     contraction), so the adjusted logit is that of the written formula.
 //   * Largest logit and sum of exponentials are kept per thread, the sum
@@ -55,10 +63,9 @@ enum { kProcess = 0, kGreedy = 1, kDraw = 2 };
 struct LogitsParams {
   m3_logits_args a;
   int slices;  // CTAs of a row
-  int slice;   // logits of a CTA, a multiple of 32
-  int window;  // logits of a CTA at a time, a multiple of 32
+  int slice;   // places of a CTA, a multiple of 32
+  int window;  // places of a CTA at a time, a multiple of 32
   int history, wide;  // counters are needed; of 32 bits
-  int vec_in, vec_out, vec_bias;  // rows start on 16 bytes
 };
 
 __device__ __forceinline__ void logits_cluster_sync() {
@@ -168,27 +175,28 @@ struct Choice {  // of a CTA, read by the cluster's first
   int nan_id;  // first NaN, or INT_MAX
 };
 
-// A run as it lies in memory; logits past the row's end are -infinity.
+// A run as it lies in memory: elements [from, n) of it are the row's, the
+// others -infinity.  vec: whole runs start on 16 bytes.
 template <typename T>
 struct Run {
   static constexpr int kWords = sizeof(T) * kVec / 4;
   uint32_t w[kWords];
-  __device__ __forceinline__ void load(const void *row, int e, int n, int vec) {
-    const T *p = static_cast<const T *>(row) + e;
-    if (vec && n >= kVec) {
+  __device__ __forceinline__ void load(const char *at, int from, int n, bool vec) {
+    if (vec && from <= 0 && n >= kVec) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 q = reinterpret_cast<const uint4 *>(p)[i];
+        const uint4 q = reinterpret_cast<const uint4 *>(at)[i];
         w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
       }
     } else if (sizeof(T) == 2) {
-      const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+      const uint16_t *h = reinterpret_cast<const uint16_t *>(at);
+      auto get = [&](int i) -> uint32_t { return i >= from && i < n ? h[i] : 0xff80u; };
 #pragma unroll
-      for (int i = 0; i < kWords; ++i)
-        w[i] = (2 * i < n ? h[2 * i] : 0xff80u) | (uint32_t)(2 * i + 1 < n ? h[2 * i + 1] : 0xff80u) << 16;
+      for (int i = 0; i < kWords; ++i) w[i] = get(2 * i) | get(2 * i + 1) << 16;
     } else {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0xff800000u;
+      for (int i = 0; i < kWords; ++i)
+        w[i] = i >= from && i < n ? reinterpret_cast<const uint32_t *>(at)[i] : 0xff800000u;
     }
   }
   __device__ __forceinline__ void get(float (&z)[kVec]) const {
@@ -198,11 +206,13 @@ struct Run {
   }
 };
 
-__device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int bf16, int e, int n, int vec) {
-  if (!vec || n < kVec) {
+// elements [from, n) of a run to `row` + place q
+__device__ __forceinline__ void store_run(const float (&z)[kVec], char *row, int bf16, int q, int from, int n,
+                                          bool vec) {
+  if (!vec || n < kVec || from > 0) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
-      if (i < n) st_any(row, e + i, z[i], bf16 ? M3_BF16 : M3_F32);
+      if (i >= from && i < n) st_any(row, q + i, z[i], bf16 ? M3_BF16 : M3_F32);
   } else if (bf16) {
     uint32_t w[4];
 #pragma unroll
@@ -210,23 +220,24 @@ __device__ __forceinline__ void store_run(const float (&z)[kVec], void *row, int
       const __nv_bfloat162 v = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t *>(&v);
     }
-    *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(row) + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4 *>(row + (int64_t)q * 2) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(row) + e);
+    float4 *p = reinterpret_cast<float4 *>(row + (int64_t)q * 4);
     p[0] = make_float4(z[0], z[1], z[2], z[3]);
     p[1] = make_float4(z[4], z[5], z[6], z[7]);
   }
 }
 
-// What a CTA needs to adjust its logits.
+// What a CTA needs to adjust its logits.  Offsets o are in the window, places
+// q in the row.
 struct Row {
-  const float *bias;
+  const float *bias;       // of place 0
   const uint32_t *seen;    // the window's bitmap, or NULL without a history
   const uint32_t *counts;  // its counters
   float rep, pres, freq;
-  int wide, vec_bias;
+  int wide;
+  bool vec_bias;
 
-  // count of the window's logit o
   __device__ __forceinline__ uint32_t count(int o) const {
     return wide ? counts[o] : counts[o >> 1] >> ((o & 1) * 16) & 0xffffu;
   }
@@ -249,18 +260,18 @@ struct Row {
       for (int i = 0; i < kVec; ++i) z[i] = i == at ? v : z[i];
     }
   }
-  // bias and mask of the run of n logits at e; ok: its bits of the mask
-  __device__ __forceinline__ void finish(float (&z)[kVec], int e, int n, uint32_t ok) const {
+  // bias and mask of elements [from, n) of the run at place q; ok: its bits of the mask
+  __device__ __forceinline__ void finish(float (&z)[kVec], int q, int from, int n, uint32_t ok) const {
     if (bias) {
-      if (vec_bias && n >= kVec) {
-        const float4 b0 = reinterpret_cast<const float4 *>(bias + e)[0];
-        const float4 b1 = reinterpret_cast<const float4 *>(bias + e)[1];
+      if (vec_bias && n >= kVec && from <= 0) {
+        const float4 b0 = reinterpret_cast<const float4 *>(bias + q)[0];
+        const float4 b1 = reinterpret_cast<const float4 *>(bias + q)[1];
         z[0] += b0.x, z[1] += b0.y, z[2] += b0.z, z[3] += b0.w;
         z[4] += b1.x, z[5] += b1.y, z[6] += b1.z, z[7] += b1.w;
       } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-          if (i < n) z[i] += bias[e + i];
+          if (i >= from && i < n) z[i] += bias[q + i];
       }
     }
     if (ok != 0xffu) {
@@ -271,13 +282,17 @@ struct Row {
   }
 };
 
-// Marks and counts the history's tokens in [w0, w0 + n); held: the first
-// kTokens of every thread, read already (-1: not in the vocabulary).
-__device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int w0, int n,
-                                                 const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
+// Marks and counts the history's tokens in the n logits from e0; held: the
+// first kTokens of every thread, read already (INT_MIN: not in the vocabulary).
+__device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int e0, int n,
+                                             const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
   const m3_logits_args &a = p.a;
   const int tid = threadIdx.x, nt = blockDim.x;
   const int64_t at = (int64_t)row * a.tokens_stride;
+  auto token = [&](int64_t i) -> int64_t {  // outside the vocabulary: outside every window
+    const int64_t t = load_int(a.tokens, at + i, a.tokens_i64);
+    return t >= 0 && t < a.V ? t : INT_MIN;
+  };
   auto mark = [&](int64_t o) {
     if (o < 0 || o >= n) return;
     if (p.wide)
@@ -297,19 +312,20 @@ __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k)
-    if (tid + k * nt < len) mark(held[k] - w0);
+    if (tid + k * nt < len) mark((int64_t)held[k] - e0);
   for (int64_t i = tid + (int64_t)kTokens * nt; i < len; i += nt)
-    mark(load_int(a.tokens, at + i, a.tokens_i64) - w0);
+    mark(token(i) - e0);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k)
-    if (tid + k * nt < len && tid + k * nt >= prompt) count(held[k] - w0);
+    if (tid + k * nt < len && tid + k * nt >= prompt) count((int64_t)held[k] - e0);
   for (int64_t i = tid + (int64_t)kTokens * nt; i < len; i += nt)
-    if (i >= prompt) count(load_int(a.tokens, at + i, a.tokens_i64) - w0);
+    if (i >= prompt) count(token(i) - e0);
   __syncthreads();
 }
 
-template <typename T, int MODE>
+// ALIGNED: every row of logits starts on 16 bytes.
+template <typename T, int MODE, bool ALIGNED>
 __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const LogitsParams p) {
   constexpr int kLogitWarps = logit_threads<MODE>() / 32;
   extern __shared__ __align__(16) uint32_t table[];  // bitmap and counters of a window
@@ -321,13 +337,25 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   const m3_logits_args &a = p.a;
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.slices, rank = blockIdx.x % p.slices;
+  const char *logits = static_cast<const char *>(a.logits) + (int64_t)row * a.ld * sizeof(T);
+  // places of the row: logit e is place e + shift; from here on, row pointers are place 0's
+  const int shift = ALIGNED || MODE == kDraw ? 0 : (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+  const int end = a.V + shift;
+  logits -= shift * (int)sizeof(T);
+  const bool vec_in = ALIGNED || (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
   const int64_t begin = (int64_t)rank * p.slice;
-  const int lo = (int)min(begin, (int64_t)a.V), hi = (int)min(begin + p.slice, (int64_t)a.V);
+  const int lo = (int)min(begin, (int64_t)end), hi = (int)min(begin + p.slice, (int64_t)end);
   if (MODE != kProcess && tid == 0) first[0] = first[1] = INT_MAX;
 
   pdl_wait();
   pdl_trigger();
-  const char *logits = static_cast<const char *>(a.logits) + (int64_t)row * a.ld * sizeof(T);
+  char *out = nullptr;
+  bool vec_out = false;
+  if (MODE == kProcess) {
+    const int size = a.out_dtype == M3_BF16 ? 2 : 4;
+    out = static_cast<char *>(a.out) + ((int64_t)row * a.out_ld - shift) * size;
+    vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  }
   const int32_t *allowed = a.allowed ? a.allowed + (int64_t)row * a.allowed_stride : nullptr;
   Row r = {};
   int len = 0, prompt = 0, held[kTokens];
@@ -338,7 +366,7 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
     for (int k = 0; k < kTokens; ++k) {
       const int i = tid + k * nt;
       const int64_t t = i < a.T ? load_int(a.tokens, at + i, a.tokens_i64) : -1;
-      held[k] = t >= 0 && t < a.V ? (int)t : -1;
+      held[k] = t >= 0 && t < a.V ? (int)t : INT_MIN;
     }
     r.rep = a.repetition ? a.repetition[row] : a.repetition_value;
     r.pres = a.presence ? a.presence[row] : a.presence_value;
@@ -349,8 +377,8 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
     prompt = (int)min(max(m, (int64_t)0), (int64_t)len);
     if (len > 0) r.seen = table, r.counts = table + p.window / 32;
   }
-  r.bias = a.bias ? a.bias + (int64_t)row * a.bias_stride : nullptr;
-  r.wide = p.wide, r.vec_bias = p.vec_bias;
+  r.bias = a.bias ? a.bias + (int64_t)row * a.bias_stride - shift : nullptr;
+  r.wide = p.wide, r.vec_bias = (reinterpret_cast<uintptr_t>(r.bias) & 15) == 0;
   float temp = 1.f;
   bool drawn = false;
   RowNoise noise = {};
@@ -367,21 +395,39 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
   if (MODE != kProcess) __syncthreads();  // `first` stands
 
-  // a run and the mask's word it lies in, as they are in memory: nothing is
-  // computed from them here, so that the loads wait for none before them
-  auto fetch = [&](Run<T> &q, uint32_t &word, int e, int n) {
-    if (n <= 0) return;
-    q.load(logits, e, n, p.vec_in);
-    word = allowed ? (uint32_t)allowed[e >> 5] : 0xffffffffu;
+  // A run and the mask's words it lies in, as they are in memory: nothing is
+  // computed from them here, so that the loads wait for none before them.
+  struct Held {
+    Run<T> run;
+    uint32_t m0, m1;
   };
-  // the run at window offset o, adjusted (again, for a closer look)
-  auto look_at = [&](float (&z)[kVec], int w0, int wn, int o) {
-    Run<T> q;
-    uint32_t word = 0u;
-    fetch(q, word, w0 + o, wn - o);
-    q.get(z);
+  auto fetch = [&](Held &h, int q, int n) {
+    if (n <= 0) return;
+    h.run.load(logits + (int64_t)q * sizeof(T), ALIGNED || MODE == kDraw ? 0 : shift - q, n, vec_in);
+    if (allowed) {
+      const int e = q - shift;
+      h.m0 = (uint32_t)allowed[max(e, 0) >> 5];
+      if (shift) h.m1 = (uint32_t)allowed[min(e + kVec - 1, a.V - 1) >> 5];
+    }
+  };
+  // the first element of the run at place q that is the row's
+  auto from = [&](int q) { return ALIGNED || MODE == kDraw ? 0 : shift - q; };
+  // the mask's bits of the run at place q
+  auto bits = [&](const Held &h, int q) -> uint32_t {
+    if (!allowed) return 0xffu;
+    const int e = q - shift;  // before the row's first logit in its first run
+    return (e < 0 ? h.m0 << -e : shift ? __funnelshift_r(h.m0, h.m1, e & 31) : h.m0 >> (e & 31)) & 0xffu;
+  };
+  // z, the run at place q (window offset o), adjusted
+  auto adjust = [&](float (&z)[kVec], uint32_t ok, int q, int o, int n) {
     r.penalize(z, o, r.hits(o));
-    r.finish(z, w0 + o, wn - o, word >> (o & 31) & 0xffu);
+    r.finish(z, q, from(q), n, ok);
+  };
+  auto look_at = [&](float (&z)[kVec], int w0, int wn, int o) {
+    Held h;
+    fetch(h, w0 + o, wn - o);
+    h.run.get(z);
+    adjust(z, bits(h, w0 + o), w0 + o, o, wn - o);
   };
 
   const int step = nt * kVec;
@@ -390,13 +436,12 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   int id = INT_MAX, nan_id = INT_MAX;
   for (int w0 = lo; w0 < hi; w0 += p.window) {
     const int wn = min(p.window, hi - w0);
-    Run<T> next[kRuns];
-    uint32_t next_word[kRuns];
+    Held next[kRuns];
 #pragma unroll
-    for (int u = 0; u < kRuns; ++u) fetch(next[u], next_word[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
+    for (int u = 0; u < kRuns; ++u) fetch(next[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
     if (r.seen) {
       if (w0 > lo) __syncthreads();  // the table has been read
-      mark_history(p, row, len, prompt, w0, wn, held, table, table + p.window / 32);
+      mark_history(p, row, len, prompt, w0 - shift, wn, held, table, table + p.window / 32);
     }
     float high = -CUDART_INF_F, mass = 0.f;  // this thread's largest of the window, the sum relative to it
     int high_at = 0;                         // the run it is in
@@ -416,14 +461,12 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
         const int o = o0 + u * step, n = wn - o;
         if (n <= 0) continue;
         float z[kVec];
-        next[u].get(z);
-        const uint32_t ok = next_word[u] >> (o & 31) & 0xffu;
-        fetch(next[u], next_word[u], w0 + o + kRuns * step, n - kRuns * step);
-        r.penalize(z, o, r.hits(o));
-        r.finish(z, w0 + o, n, ok);
+        next[u].run.get(z);
+        const uint32_t ok = bits(next[u], w0 + o);
+        fetch(next[u], w0 + o + kRuns * step, n - kRuns * step);
+        adjust(z, ok, w0 + o, o, n);
         if (MODE == kProcess) {
-          store_run(z, static_cast<char *>(a.out) + (int64_t)row * a.out_ld * (a.out_dtype == M3_BF16 ? 2 : 4),
-                    a.out_dtype == M3_BF16, w0 + o, n, p.vec_out);
+          store_run(z, out, a.out_dtype == M3_BF16, w0 + o, from(w0 + o), n, vec_out);
           continue;
         }
         float m = -CUDART_INF_F;
@@ -463,7 +506,7 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
       int at = INT_MAX;
 #pragma unroll
       for (int i = kVec - 1; i >= 0; --i)
-        if (z[i] == cta) at = w0 + high_at + i;
+        if (z[i] == cta) at = w0 + high_at + i - shift;
       atomicMin(&first[0], at);
     }
     if (bad) {
@@ -472,7 +515,7 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
         look_at(z, w0, wn, o);
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
-          if (z[i] != z[i]) atomicMin(&first[1], w0 + o + i);
+          if (z[i] != z[i]) atomicMin(&first[1], w0 + o + i - shift);
       }
     }
     if (MODE == kDraw && drawn && cta > -CUDART_INF_F) {
@@ -593,11 +636,7 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   if (p.slices > 1) logits_cluster_sync();  // no CTA leaves while its choice is read
 }
 
-bool rows_on_16(const void *p, int64_t ld, int B, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (B == 1 || ld * size % 16 == 0);
-}
-
-template <typename T, int MODE>
+template <typename T, int MODE, bool ALIGNED>
 cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   LogitsParams p = {};
   p.a = a;
@@ -605,9 +644,6 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
               (a.repetition || a.presence || a.frequency || a.repetition_value != 1.f || a.presence_value != 0.f ||
                a.frequency_value != 0.f);
   p.wide = a.T > kCountMax;
-  p.vec_in = rows_on_16(a.logits, a.ld, a.B, sizeof(T));
-  p.vec_out = a.out && rows_on_16(a.out, a.out_ld, a.B, a.out_dtype == M3_BF16 ? 2 : 4);
-  p.vec_bias = a.bias && rows_on_16(a.bias, a.bias_stride, a.B, 4);
   // CTAs of a row: what fills two CTAs an SM, at least one run a thread each;
   // those that have to meet are a cluster, a power of two up to 8
   constexpr int kLogitThreads = logit_threads<MODE>();
@@ -620,12 +656,13 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   } else {
     p.slices = want;
   }
-  p.slice = (int)(((int64_t)a.V + p.slices - 1) / p.slices + 31) / 32 * 32;
+  const int places = a.V + (ALIGNED || MODE == kDraw ? 0 : kVec - 1);  // wherever the rows start
+  p.slice = ((places + p.slices - 1) / p.slices + 31) / 32 * 32;
   p.window = p.history ? min(p.slice, p.wide ? kWindow / 2 : kWindow) : p.slice;
   const int64_t grid = (int64_t)a.B * p.slices;
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
   const int threads = min(kLogitThreads, ((p.slice + kVec - 1) / kVec + 31) / 32 * 32);
-  auto kern = logits_kernel<T, MODE>;
+  auto kern = logits_kernel<T, MODE, ALIGNED>;
   const size_t smem = p.history ? (size_t)p.window / 8 + (size_t)p.window * (p.wide ? 4 : 2) : 0;
   static LaunchCache cache;
   if (cudaError_t e = ensure_smem_optin(cache, kern, kWindow / 8 + kWindow * 2); e != cudaSuccess) return e;
@@ -647,19 +684,25 @@ cudaError_t launch_logits_t(const m3_logits_args &a, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+template <typename T, int MODE>
+cudaError_t launch_logits_a(const m3_logits_args &a, cudaStream_t stream) {
+  const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (a.B == 1 || a.ld * sizeof(T) % 16 == 0);
+  return aligned ? launch_logits_t<T, MODE, true>(a, stream) : launch_logits_t<T, MODE, false>(a, stream);
+}
+
+template <int MODE>
+cudaError_t launch_logits(const m3_logits_args &a, cudaStream_t stream) {
+  return a.dtype == M3_BF16 ? launch_logits_a<__nv_bfloat16, MODE>(a, stream) : launch_logits_a<float, MODE>(a, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_process_logits(const m3_logits_args &a, cudaStream_t stream) {
-  return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kProcess>(a, stream)
-                            : launch_logits_t<float, kProcess>(a, stream);
+  return launch_logits<kProcess>(a, stream);
 }
 
 cudaError_t launch_next_tokens(const m3_logits_args &a, cudaStream_t stream) {
-  if (a.sample)
-    return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kDraw>(a, stream)
-                              : launch_logits_t<float, kDraw>(a, stream);
-  return a.dtype == M3_BF16 ? launch_logits_t<__nv_bfloat16, kGreedy>(a, stream)
-                            : launch_logits_t<float, kGreedy>(a, stream);
+  return a.sample ? launch_logits<kDraw>(a, stream) : launch_logits<kGreedy>(a, stream);
 }
 
 }  // namespace m3
