@@ -183,26 +183,27 @@ __device__ __forceinline__ void w4_block(const W4Params &p, float (&tot)[MT][NT]
 
 constexpr int kW4SmemBudget = 227 * 1024;  // x and the partial sums: all an SM gives a CTA
 
-// The shape of a CTA by its batch tiles MT.  One tile: as many warps as the
-// SM takes, which the chain unpack - MMA - scale of a block needs.  Two: two
-// row blocks a warp, which share the batch operand's loads from shared memory
-// (50,280 x 2,560, 16 rows: 26.6 against 32.0 us with one).  Four: one row
-// block and 16 warps (64 rows of 9,440 x 2,048: 13.9 against 16.5 us with two
-// and 12).  Finer groups hold more scales in flight: fewer warps, one block.
-template <int MT, int GPT>
+// The shape of a CTA by its batch tiles MT and the row blocks NT of a warp.
+// One tile: as many warps as the SM takes, which the chain unpack - MMA -
+// scale of a block needs.  Two: two row blocks a warp, which share the batch
+// operand's loads from shared memory, where that still leaves a row block to
+// every SM (50,280 x 2,560, 16 rows: 26.6 against 32.0 us with one; 2,048 x
+// 4,096 has 128 row blocks: 7.1 against 6.0 us).  Four: one row block and 16
+// warps (64 rows of 9,440 x 2,048: 13.9 against 16.5 us with two and 12).
+// Finer groups hold more scales in flight: fewer warps, one block.
+template <int MT, int NT, int GPT>
 struct W4Shape {
   static constexpr int kWarps = MT == 1 ? (GPT == 1 ? 32 : GPT == 2 ? 24 : 16) : 16;
-  static constexpr int NT = MT == 2 && GPT != 4 ? 2 : 1;
-  static constexpr int kDepth = 2;                         // blocks a warp has in flight: 48 KB an SM or more
+  static constexpr int kDepth = 2;                         // blocks a warp has in flight: 32 KB an SM or more
   static constexpr int kLd = NT * 16 + 1;                  // partial sums of a batch row, padded against conflicts
   static constexpr int kRed = MT * 8 * kLd;                // partial sums of a warp
   static constexpr int kBufs = MT == 4 ? 1 : 2;            // of them: a second one saves a barrier, x wants the room
 };
 
 // x as the MMAs take it: [tile][run j][batch tile][term][lane] pieces of 16 bytes
-template <int MT, int GPT, int TERMS>
+template <typename S, int MT, int TERMS>
 int64_t w4_stream_smem(int tiles, int wk, int wn) {
-  return (int64_t)tiles * 4 * MT * TERMS * 512 + (int64_t)W4Shape<MT, GPT>::kBufs * wk * wn * W4Shape<MT, GPT>::kRed * 4;
+  return (int64_t)tiles * 4 * MT * TERMS * 512 + (int64_t)S::kBufs * wk * wn * S::kRed * 4;
 }
 
 // The decode batches' kernel: persistent CTAs that hold all of x in shared
@@ -211,11 +212,11 @@ int64_t w4_stream_smem(int tiles, int wk, int wn) {
 // row blocks in turn, its warps the tiles kt = wk, wk + p.wk, ... of them, and
 // their sums are added in warp order through shared memory, behind a barrier
 // of the group.
-template <typename XT, int MT, int GPT, bool ZEROS>
-__global__ void __launch_bounds__(W4Shape<MT, GPT>::kWarps * 32, 1) w4_stream_kernel(const W4Params p) {
+template <typename XT, int MT, int NT, int GPT, bool ZEROS>
+__global__ void __launch_bounds__(W4Shape<MT, NT, GPT>::kWarps * 32, 1) w4_stream_kernel(const W4Params p) {
   using X = W4X<XT>;
-  using S = W4Shape<MT, GPT>;
-  constexpr int TERMS = X::kTerms, NT = S::NT, RED = S::kRed, DEPTH = S::kDepth, ROWS = NT * 16, LD = S::kLd;
+  using S = W4Shape<MT, NT, GPT>;
+  constexpr int TERMS = X::kTerms, RED = S::kRed, DEPTH = S::kDepth, ROWS = NT * 16, LD = S::kLd;
   extern __shared__ __align__(16) uint4 w4_smem[];
   const int pieces = p.tiles * 4 * MT * 32;
   float *red = reinterpret_cast<float *>(w4_smem + (int64_t)pieces * TERMS);
@@ -432,13 +433,13 @@ cudaError_t launch_w4_direct(const W4Params &p, cudaStream_t stream) {
 // Warps along K: the split with the fewest steps of the busiest warp (fewest
 // warps a row block on ties: less to add up), then as many row blocks per CTA
 // as keep every SM busy.
-template <typename XT, int MT, int GPT, bool ZEROS>
+template <typename XT, int MT, int NT, int GPT, bool ZEROS>
 cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
-  using S = W4Shape<MT, GPT>;
+  using S = W4Shape<MT, NT, GPT>;
   constexpr int TERMS = W4X<XT>::kTerms, WARPS = S::kWarps;
   p.mtiles = (p.M + MT * 8 - 1) / (MT * 8);
   const int sms = max(1, sm_count_current() / p.mtiles);  // of a batch tile
-  const int rbs = (p.blocks + S::NT - 1) / S::NT;
+  const int rbs = (p.blocks + NT - 1) / NT;
   int64_t best = INT64_MAX;
   for (int wk = (WARPS + 15) / 16; wk <= WARPS; wk *= 2) {  // at most 16 groups: a barrier each
     const int64_t streams = (int64_t)sms * (WARPS / wk);
@@ -446,10 +447,10 @@ cudaError_t launch_w4_stream(W4Params p, cudaStream_t stream, bool *taken) {
     if (steps < best) best = steps, p.wk = wk;
   }
   p.wn = min(WARPS / p.wk, (rbs + sms - 1) / sms);
-  const int64_t smem = w4_stream_smem<MT, GPT, TERMS>(p.tiles, p.wk, p.wn);
+  const int64_t smem = w4_stream_smem<S, MT, TERMS>(p.tiles, p.wk, p.wn);
   *taken = smem <= kW4SmemBudget;
   if (!*taken) return cudaSuccess;
-  auto kern = w4_stream_kernel<XT, MT, GPT, ZEROS>;
+  auto kern = w4_stream_kernel<XT, MT, NT, GPT, ZEROS>;
   static LaunchCache cache;
   if (cudaError_t e = ensure_smem_optin(cache, kern, kW4SmemBudget); e != cudaSuccess) return e;
   const int64_t grid = (int64_t)min(sms, (rbs + p.wn - 1) / p.wn) * p.mtiles;
@@ -462,9 +463,13 @@ cudaError_t launch_w4_x(const W4Params &p, cudaStream_t stream) {
   bool taken = false;
   cudaError_t e = cudaSuccess;
   // the largest batch tile whose x fits in shared memory
-  if (p.M > 16) e = launch_w4_stream<XT, 4, GPT, ZEROS>(p, stream, &taken);
-  if (!taken && e == cudaSuccess && p.M > 8) e = launch_w4_stream<XT, 2, GPT, ZEROS>(p, stream, &taken);
-  if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 1, GPT, ZEROS>(p, stream, &taken);
+  if (p.M > 16) e = launch_w4_stream<XT, 4, 1, GPT, ZEROS>(p, stream, &taken);
+  if (!taken && e == cudaSuccess && p.M > 8) {
+    if constexpr (GPT != 4)
+      if (p.blocks >= 2 * sm_count_current()) e = launch_w4_stream<XT, 2, 2, GPT, ZEROS>(p, stream, &taken);
+    if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 2, 1, GPT, ZEROS>(p, stream, &taken);
+  }
+  if (!taken && e == cudaSuccess) e = launch_w4_stream<XT, 1, 1, GPT, ZEROS>(p, stream, &taken);
   if (taken || e != cudaSuccess) return e;
   return p.M <= 8 ? launch_w4_direct<XT, 1, GPT, ZEROS>(p, stream) : launch_w4_direct<XT, 4, GPT, ZEROS>(p, stream);
 }
