@@ -424,3 +424,18 @@ def test_infinite_temperature_is_uniform():
     count = torch.bincount(ids.cpu(), minlength=8)
     assert not count[4:].any() and bool(((count[:4] - 500.0).abs() <= 5 * (2000 * 0.25 * 0.75) ** 0.5).all())
     torch.testing.assert_close(lp, torch.full_like(lp, -math.log(4.0)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [20000, 20003])
+def test_in_place_of_many_rows(V, dtype):
+    """Seen logits are read before any thread stores over them."""
+    for T in (30, 1500, 6000):
+        a = case(300, V, T, dtype, seed=T, mask="shared")
+        want = process_logits(**a)
+        for _ in range(3):
+            b = dict(a, logits=a["logits"].clone())
+            assert torch.equal(process_logits(**b, out=b["logits"]), want)
+        small = {k: v[:3] if v.shape[0] == 300 else v for k, v in a.items()}
+        check_process(small)
+        check_next(small)
