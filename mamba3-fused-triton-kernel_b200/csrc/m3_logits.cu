@@ -133,11 +133,13 @@ struct Drawn {
 };
 
 // Whether a beats b: by the difference of the two, in 64 bits, so that large
-// logits do not swallow the noise.  Of two infinite ones b stays.
+// logits do not swallow the noise, and times the temperature, which is above
+// 0 (a product where a quotient of 64 bits takes ten times as long).  Of two
+// infinite ones b stays.
 __device__ __forceinline__ bool draw_beats(const Drawn &a, const Drawn &b, float temperature) {
   if (b.id == INT_MAX) return a.id != INT_MAX;
   if (a.id == INT_MAX) return false;
-  const double d = ((double)a.z - (double)b.z) / (double)temperature + (a.g - b.g);
+  const double d = fma(a.g - b.g, (double)temperature, (double)a.z - (double)b.z);
   return d > 0.0 || (d == 0.0 && a.id < b.id);
 }
 
@@ -153,6 +155,7 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 __device__ __forceinline__ Drawn warp_best(Drawn b, float temperature) {
+  if (!__any_sync(kFullMask, b.id != INT_MAX)) return b;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Drawn c = {__shfl_xor_sync(kFullMask, b.g, o), __shfl_xor_sync(kFullMask, b.z, o),

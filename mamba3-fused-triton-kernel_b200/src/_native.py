@@ -226,8 +226,12 @@ def host_entry(name: str):
             return _no_host
         lib = load()
         spec = importlib.util.spec_from_file_location("m3_host", HOST_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise RuntimeError(f"{HOST_PATH} does not fit this PyTorch ({e}); run "
+                               "`python mamba3-fused-triton-kernel_b200/build_native.py --force`") from e
         module.bind(*(ctypes.cast(getattr(lib, f), c_void_p).value
                       for f in ("m3_linear_w4", "m3_process_logits", "m3_next_tokens")))
         _host = module
