@@ -146,17 +146,18 @@ class W4Projection:
     count (through ``.data``) needs ``refresh()``.  Quantising waits for the
     GPU: it belongs before a capture."""
 
-    __slots__ = ("weight", "group_size", "key", "w4")
+    __slots__ = ("weight", "group_size", "source", "key", "w4")
 
     def __init__(self, weight, group_size: int):
         _check_group(group_size)
         self.weight, self.group_size = weight, group_size  # weight: a callable, the current parameter
-        self.key = self.w4 = None
+        self.source = self.key = self.w4 = None
         self.get()
 
     def get(self) -> W4Weight:
         w = self.weight()
-        if self.key != (w.data_ptr(), w._version, w.dtype):
+        # the parameter itself is held, so that no other can be taken for it
+        if w is not self.source or self.key != (w._version, w.data_ptr(), w.dtype):
             self.refresh()
         return self.w4
 
@@ -172,7 +173,7 @@ class W4Projection:
             old.scales.copy_(new.scales)
         else:
             self.w4 = new
-        self.key = (w.data_ptr(), w._version, w.dtype)
+        self.source, self.key = w, (w._version, w.data_ptr(), w.dtype)
 
 
 _host = None  # the host module's linear_w4, once looked up

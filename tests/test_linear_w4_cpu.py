@@ -142,3 +142,30 @@ def test_abi_null_block():
     assert nat.load().m3_linear_w4(None, None) == nat.M3_ERR_NULL
     assert isinstance(ctypes.c_char_p(_w4()).value, bytes)
     assert W4Weight._fields == ("codes", "scales", "zeros", "group_size", "in_features")
+
+
+def test_projection_follows_its_weight():
+    """A change in place, another parameter on the same memory, another shape,
+    and one that is not counted."""
+    from src.kernels.linear_w4 import W4Projection
+    lin = torch.nn.Linear(256, 48, bias=False)
+    p = W4Projection(lambda: lin.weight, 64)
+    first = p.get()
+    assert p.get() is first
+    want = lambda: dequantize_w4(quantize_w4(lin.weight, 64))  # noqa: E731
+    codes = first.codes.data_ptr()
+    with torch.no_grad():
+        lin.weight.mul_(-2.0)
+    assert torch.equal(dequantize_w4(p.get()), want()) and p.get().codes.data_ptr() == codes
+    other = torch.nn.Parameter(lin.weight.data)
+    other.data.mul_(3.0)
+    lin.weight = other
+    assert torch.equal(dequantize_w4(p.get()), want())
+    lin.weight.data.mul_(0.5)
+    p.refresh()
+    assert torch.equal(dequantize_w4(p.get()), want())
+    lin.weight = torch.nn.Parameter(torch.randn(16, 128))
+    assert p.get().shape == (16, 128) and torch.equal(dequantize_w4(p.get()), want())
+    lin.weight = torch.nn.Parameter(torch.randn(16, 128).half())
+    with pytest.raises(ValueError):
+        p.get()
