@@ -141,10 +141,11 @@ class W4Projection:
     """The 4-bit form of one projection of a model, for a decoder.
 
     ``get()`` quantises the weight when first called, and again, into the
-    same tensors (so that a captured graph sees the change), once the weight
-    has been replaced or modified in place.  A change that PyTorch does not
-    count (through ``.data``) needs ``refresh()``.  Quantising waits for the
-    GPU: it belongs before a capture."""
+    same tensors, once the weight has been replaced or modified in place.  A
+    change that PyTorch does not count (through ``.data``) needs
+    ``refresh()``.  A captured graph replays what the tensors hold: it sees a
+    change after the next ``get()``.  Quantising waits for the GPU: it belongs
+    before a capture."""
 
     __slots__ = ("weight", "group_size", "source", "key", "w4")
 
