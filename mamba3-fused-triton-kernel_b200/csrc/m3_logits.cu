@@ -287,6 +287,7 @@ struct Row {
 
 // Marks and counts the history's tokens in the n logits from e0; held: the
 // first kTokens of every thread, read already (INT_MIN: not in the vocabulary).
+// The bitmap is clear.
 __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int len, int prompt, int e0, int n,
                                              const int (&held)[kTokens], uint32_t *seen, uint32_t *counts) {
   const m3_logits_args &a = p.a;
@@ -311,8 +312,6 @@ __device__ __forceinline__ void mark_history(const LogitsParams &p, int row, int
     else
       atomicAdd(&counts[o >> 1], 1u << ((o & 1) * 16));
   };
-  for (int i = tid; i < p.window / 32; i += nt) seen[i] = 0u;
-  __syncthreads();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k)
     if (tid + k * nt < len) mark((int64_t)held[k] - e0);
@@ -349,6 +348,10 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   const int64_t begin = (int64_t)rank * p.slice;
   const int lo = (int)min(begin, (int64_t)end), hi = (int)min(begin + p.slice, (int64_t)end);
   if (MODE != kProcess && tid == 0) first[0] = first[1] = INT_MAX;
+  auto clear = [&] {
+    for (int i = tid; i < p.window / 32; i += nt) table[i] = 0u;
+  };
+  if (p.history) clear();  // while the preceding kernel runs
 
   pdl_wait();
   pdl_trigger();
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
   // exponents are taken to base 2; kept finite and above 0, so that -infinity stays it
   const float scale = fmaxf(fminf(kLog2e / temp, FLT_MAX), FLT_MIN);
   auto bound = [&](float v, uint32_t w) { return fmaf(v, scale, -noise_log2(w)); };
-  if (MODE != kProcess) __syncthreads();  // `first` stands
+  __syncthreads();  // `first` stands, the bitmap is clear
 
   // A run and the mask's words it lies in, as they are in memory: nothing is
   // computed from them here, so that the loads wait for none before them.
@@ -443,7 +446,11 @@ __global__ void __launch_bounds__(logit_threads<MODE>(), 2) logits_kernel(const 
 #pragma unroll
     for (int u = 0; u < kRuns; ++u) fetch(next[u], w0 + tid * kVec + u * step, wn - tid * kVec - u * step);
     if (r.seen) {
-      if (w0 > lo) __syncthreads();  // the table has been read
+      if (w0 > lo) {
+        __syncthreads();  // the table has been read
+        clear();
+        __syncthreads();
+      }
       mark_history(p, row, len, prompt, w0 - shift, wn, held, table, table + p.window / 32);
     }
     float high = -CUDART_INF_F, mass = 0.f;  // this thread's largest of the window, the sum relative to it
