@@ -454,8 +454,9 @@ int m3_device_error(int reset) {
   const int d = m3::mimo_stream_device_error(reset != 0);
   const int e = m3::gemm_device_error(reset != 0);
   const int f = m3::siso_prefill_device_error(reset != 0);
-  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0) return -1;
-  return a | b | c | d | e | f;
+  const int g = m3::w4_device_error(reset != 0);
+  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0 || g < 0) return -1;
+  return a | b | c | d | e | f | g;
 }
 
 int m3_selftest_wait_timeout(m3_stream_t stream) {

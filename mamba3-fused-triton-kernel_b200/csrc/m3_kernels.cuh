@@ -540,6 +540,7 @@ int mimo_device_error(bool reset);
 int mimo_stream_device_error(bool reset);
 int siso_prefill_device_error(bool reset);
 int gemm_device_error(bool reset);
+int w4_device_error(bool reset);
 
 // Heads handled by one CTA of the MIMO kernels.
 int mimo_heads_per_cta(int H);

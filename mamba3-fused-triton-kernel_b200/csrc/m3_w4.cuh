@@ -106,4 +106,8 @@ __device__ __forceinline__ void w4_store(const W4Params &p, int m, int n, float 
     static_cast<float *>(p.y)[(int64_t)m * p.ldy + n] = s;
 }
 
+// The kernel for many batch rows of a bf16 x (m3_w4_tc.cu); not taken: x is
+// laid out as TMA does not read it.
+cudaError_t launch_w4_tc(const W4Params &p, int group, cudaStream_t stream, bool *taken);
+
 }  // namespace m3

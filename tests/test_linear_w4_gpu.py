@@ -214,3 +214,93 @@ def test_host_module_and_python_path_agree(monkeypatch):
         assert host(*args) is None
     monkeypatch.setattr(mod, "_host", nat._no_host)
     assert torch.equal(linear_w4(x, w.codes, w.scales, w.zeros, group_size=64), y)
+
+
+# more than 32 batch rows of a weight large enough for the tensor memory path:
+# ragged rows and columns, one and several items a CTA, split K
+MANY = [(40, 9000, 1200), (64, 50000, 264), (33, 9440, 2048), (65, 4225, 1160), (130, 20001, 136), (300, 1000, 2560),
+        (513, 2048, 520), (2200, 17, 8200), (128, 2048, 4096), (1000, 9440, 384)]
+
+
+@pytest.mark.parametrize("M,N,K", MANY)
+@pytest.mark.parametrize("G", GROUP_SIZES)
+def test_many_rows(M, N, K, G):
+    from src import _native as nat
+    for zeros, s_dtype in ((False, torch.float32), (True, torch.bfloat16)):
+        w = make(N, K, G, zeros, s_dtype, seed=M + N + K)
+        g = torch.Generator(device="cuda").manual_seed(K)
+        x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+        for out_dtype in (torch.float32, torch.bfloat16):
+            check(linear_w4(x, w.codes, w.scales, w.zeros, group_size=G, out_dtype=out_dtype), x, w)
+    assert nat.load().m3_device_error(0) == 0
+
+
+def test_many_rows_of_other_layouts():
+    """Strided rows behind whose end NaN stands; rows off 16 bytes, of an odd
+    length or the same row (not read by TMA); fp32."""
+    w = make(9440, 1160, 64, True)
+    wide = torch.full((200, 1280), float("nan"), device="cuda").bfloat16()
+    wide[:, 8:1168] = torch.randn(200, 1160, device="cuda")
+    shifted = torch.full((200, 1280), float("nan"), device="cuda").bfloat16()
+    shifted[:, 3:1163] = wide[:, 8:1168]
+    for x in (wide[:, 8:1168], wide[::2, 8:1168], shifted[:, 3:1163], wide[:1, 8:1168].expand(100, 1160),
+              wide[:100, 8:1168].float()):
+        check(linear_w4(x, w.codes, w.scales, w.zeros, group_size=64), x, w)
+    w = make(9440, 1111, 128, False)
+    x = torch.randn(70, 1111, device="cuda").bfloat16()
+    check(linear_w4(x, w.codes, w.scales), x, w)
+
+
+def test_many_rows_not_finite():
+    """A row of x or of the scales that is not finite stays in its row or
+    column, also where the last rows and groups are not whole."""
+    w = make(9001, 1032, 128, False)
+    x = torch.randn(130, 1032, device="cuda").bfloat16()
+    want = linear_w4(x, w.codes, w.scales)
+    x[7], x[129, 0] = float("nan"), float("inf")
+    scales = w.scales.clone()
+    scales[5], scales[9000] = float("inf"), float("nan")
+    y = linear_w4(x, w.codes, scales)
+    rows, cols = torch.ones(130, dtype=torch.bool, device="cuda"), torch.ones(9001, dtype=torch.bool, device="cuda")
+    rows[7] = rows[129] = False
+    cols[5] = cols[9000] = False
+    assert torch.equal(y[rows][:, cols], want[rows][:, cols])
+    assert bool(y[7].isnan().all()) and not bool(y[129].isfinite().any())
+    assert bool(y[:, 9000].isnan().all()) and not bool(y[:, 5].isfinite().any())
+
+
+def test_many_rows_same_bits_streams_and_graphs():
+    w = [make(9440, 1032, 32, True, seed=i) for i in range(2)]
+    x = torch.randn(100, 1032, device="cuda").bfloat16()
+    want = [linear_w4(x, v.codes, v.scales, v.zeros, group_size=32) for v in w]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got += [(i, linear_w4(x, w[i].codes, w[i].scales, w[i].zeros, group_size=32)) for i in (0, 1, 0, 1)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    graphs, outs = [], []
+    for v in w:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(linear_w4(x, v.codes, v.scales, v.zeros, group_size=32))
+        graphs.append(graph)
+    x.copy_(torch.randn(100, 1032, device="cuda"))
+    for graph, s in zip(graphs, streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    for y, v in zip(outs, w):
+        check(y, x, v)
+
+
+def test_many_rows_weight_written_just_before():
+    x = torch.randn(64, 2048, device="cuda").bfloat16()
+    w = [make(9440, 2048, 128, True, seed=i) for i in range(2)]
+    buf = W4Weight(*(t.clone() if isinstance(t, torch.Tensor) else t for t in w[0]))
+    want = [linear_w4(x, v.codes, v.scales, v.zeros) for v in w]
+    for i in (1, 0, 1, 0):
+        buf.scales.copy_(w[i].scales), buf.zeros.copy_(w[i].zeros), buf.codes.copy_(w[i].codes)
+        assert torch.equal(linear_w4(x, buf.codes, buf.scales, buf.zeros), want[i])
