@@ -502,14 +502,16 @@ cudaError_t launch_linear_w4(const m3_w4_args &a, cudaStream_t stream) {
   p.zeros = a.zeros, p.z_ld = a.zero_stride;
   p.y = a.y, p.ldy = a.ldy, p.y_bf16 = a.y_dtype == M3_BF16;
   // Many rows of a bf16 x go to the tensor memory path once there are some 30
-  // blocks and 64 batch rows of work for an SM: us against the kernels here,
-  // G 128, 50,280 x 2,560, 64 rows 40 / 72, 256 rows 86 / 204; 9,440 x 2,048,
-  // 64 rows 11.6 / 13.9; 2,048 x 4,096, 64 rows 10.1 / 10.7, with 27.7 blocks
-  // an SM; 4,224 x 1,024 (14.3), 64 rows 7.3 / 5.7, 128 rows 8.8 / 8.4.  Up to
-  // 32 rows it is within a few percent at the large weight, slower elsewhere
-  // (9,440 x 2,048: 11.3 / 9.3).
-  if (a.x_dtype == M3_BF16 && a.M > 32 &&
-      (int64_t)p.blocks * p.tiles * ((a.M + 63) / 64) >= 30ll * sm_count_current()) {
+  // blocks and 64 batch rows of work for an SM: us there / with the kernels
+  // here, G 128, 50,280 x 2,560, 64 rows 31 / 72, 256 rows 78 / 204; 9,440 x
+  // 2,048, 64 rows 11.2 / 13.9; 4,096 x 2,048 (27.7 blocks an SM), 64 rows
+  // 8.8 / 8.8; 4,224 x 1,024 (14.3), 64 rows 7.3 / 5.7, 128 rows 8.8 / 8.4.  17
+  // to 32 rows take more work, and groups of 128, whose sums are read back
+  // least often: 32 rows of 50,280 x 2,560 31 / 42, of 9,440 x 2,048 11.0 / 9.3;
+  // with groups of 64 48 / 44.
+  const int64_t work = (int64_t)p.blocks * p.tiles * ((a.M + 63) / 64);
+  if (a.x_dtype == M3_BF16 && ((a.M > 32 && work >= 30ll * sm_count_current()) ||
+                               (a.M > 16 && a.group == 128 && work >= 150ll * sm_count_current()))) {
     bool taken = false;
     if (cudaError_t e = launch_w4_tc(p, a.group, stream, &taken); taken || e != cudaSuccess) return e;
   }

@@ -9,32 +9,37 @@
 // thread unpacks one row: 64 bytes of codes are the 64 32-bit columns of a
 // 128-column tile, in order.
 //
-//   warps 0-15   read D (TMEM lanes 32 (w % 4) .. + 31: the thread's weight
-//                row, a quarter of the batch rows each), times the row's
-//                scale into registers, store at the end
-//   warps 16-23  unpack: warp w takes lanes 32 (w % 4) .. of every other
-//                tile, and fetches their scales into shared memory
-//   warp 24      lane 0: copies of codes into a ring of tiles
-//   warp 25      lane 0: copies of x likewise
-//   warps 26-27  lane 0: the MMAs, an accumulator each; the first allocates
-//                TMEM
+//   readers      8 or 16 warps: D (TMEM lanes 32 (w % 4) .. + 31: the
+//                thread's weight row, a share of the batch rows each), times
+//                the row's scale into registers, stored at the end
+//   unpackers    the other 16 or 8 of the first 24 warps, in sets of four
+//                that take the tiles in turn: warp w of a set the rows of
+//                lanes 32 (w % 4) .., and their scales into shared memory
+//   warp 24      one lane: copies of codes into a ring of tiles
+//   warp 25      one lane: copies of x likewise
+//   warps 26-27  one lane each: the MMAs of every other group; the first
+//                allocates TMEM
 //
-// What bounds it is the hand-overs.  A tile's MMAs take 512 cycles (NB 128);
-// a tcgen05.commit holds the thread that issues it for about 285, hence two
-// such threads and two commits a tile; with one thread, three commits and 8
-// reading warps that held 64 columns a tile took 2,250 cycles, now 1,200.
-// Scales read by every reader from global memory cost 170 of them.
-// 9,440 x 2,048, G 128: 256 rows 14.6 us, 4,096 rows 181 us (53 % of the
-// tensor memory path's rate in the library's bf16 product, which reads an
-// unquantised weight); 50,280 x 2,560, 64 rows 40 us.  Groups of 32 read D
-// four times as often: 29 us for the 14.6.
+// What bounds it is the hand-overs and the issue of MMAs and commits, about
+// 90 and 300 cycles each, hence two warps for them and few commits: a tile's
+// MMAs take 512 cycles (NB 128), the kernel 1,150.  Steps, 1,024 rows of 9,440
+// x 2,048: one MMA warp, three commits a tile, 8 readers of 64 columns 89 us;
+// two, one barrier for a tile's places, 16 readers 62; scales through shared
+// memory, D read 16 columns at a time, which spills nothing 57; stores with
+// their addresses hoisted 47; elect.sync for the one lane 44 (tensor pipe
+// active 42 % of the time).  Groups of 32 read D four times as often: 99 us.
+// 64 rows of 50,280 x 2,560: 31 us (72 with the stream kernel); 256 rows of
+// 9,440 x 2,048: 14 (75).  NB is 64 up to 64 rows (46 us with 128), with 16
+// unpackers for groups of 128 and 16 readers for finer ones (73 us for groups
+// of 32, 76 the other way).
 //
-// CTAs are persistent over items of 128 weight rows by NB batch rows (64 up
-// to 64 rows: 40 against 46 us there); where there are too few of them, the
-// CTAs of a cluster split K, two tiles each or more, and their sums are added
-// in rank order through distributed shared memory.  Clusters of 8 took longer
-// than of 4 (16 x 8 CTAs of a whole SM each: 21 against 12 us).  Every
-// mbarrier wait is bounded; no copy uses cluster multicast.
+// CTAs are persistent over items of 128 weight rows by NB batch rows.  Where
+// there are too few of them and K is long, the CTAs of a cluster split K and
+// their sums are added in rank order through distributed shared memory, which
+// takes as long as about six tiles (128 rows of 4,224 x 1,024, 8 tiles: 8.3
+// with one, 8.8 us with four).  Clusters of 8 took longer than of 4 (128 rows
+// of 2,048 x 4,096: 21 against 12 us).  Every mbarrier wait is bounded; no copy
+// uses cluster multicast.
 #include <cuda.h>
 
 #include "m3_async.cuh"
@@ -49,29 +54,37 @@ constexpr int kTcRows = 128;        // weight rows of an item
 constexpr int kTcCodes = 8 * 1024;  // codes of a tile
 constexpr int kTcRing = 4;          // tiles of x, and of unpacked codes (64 TMEM columns each)
 constexpr int kTcCodeRing = 8;      // tiles of codes
-constexpr int kTcScaleRing = 8;     // tiles of scales: more than the ring and the accumulators together
-constexpr int kTcD = 2;             // accumulators, an MMA warp each
-constexpr int kTcReaders = 16, kTcUnpackers = 8;
-constexpr int kTcCopyCodes = kTcReaders + kTcUnpackers, kTcCopyX = kTcCopyCodes + 1, kTcMma = kTcCopyX + 1;
-constexpr int kTcThreads = (kTcMma + kTcD) * 32;
+constexpr int kTcMmas = 2;          // warps that issue MMAs
+constexpr int kTcCopyCodes = 24, kTcCopyX = kTcCopyCodes + 1, kTcMma = kTcCopyX + 1;
+constexpr int kTcThreads = (kTcMma + kTcMmas) * 32;
 constexpr int kTmemCols = 512;
 
 // Shared memory: x, codes, scales (128 of each of a tile's GPT groups),
 // barriers, and up to 1,024 bytes of alignment.  NB: batch rows of an item.
 template <int NB, int GPT>
 struct TcSmem {
+  static constexpr int kD = 256 / NB;  // accumulators, NB TMEM columns each
+  static constexpr int kScaleRing = 4 * kD;  // tiles of scales: more than the ring and the accumulators together
   static constexpr int kX = NB * 256;  // of a tile: two 64-column halves
   static constexpr int kCodes = kTcRing * kX, kScales = kCodes + kTcCodeRing * kTcCodes;
-  static constexpr int kBars = kScales + kTcScaleRing * GPT * kTcRows * 4;
+  static constexpr int kBars = kScales + kScaleRing * GPT * kTcRows * 4;
   static constexpr int kBytes = kBars + 512 + 1024;
-  static_assert(64 * kTcRing + NB * kTcD <= kTmemCols, "TMEM columns");
-  static_assert((3 * kTcRing + 2 * kTcCodeRing + 2 * kTcD) * 8 + 8 <= 512, "barriers");
+  static_assert(64 * kTcRing + NB * kD <= kTmemCols, "TMEM columns");
+  static_assert((3 * kTcRing + 2 * kTcCodeRing + 2 * kD) * 8 + 8 <= 512, "barriers");
   static_assert(kTcRows * NB * 4 <= kCodes, "the sums of a split K take the place of x");
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// One thread of the warp, which the compiler knows to be one: it then issues
+// tcgen05 instructions from uniform registers without a loop over threads.
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ void tc_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -169,6 +182,7 @@ template <int NB, int GPT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     w4_tc_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tcodes, const W4Params p, int cs, int items) {
   using L = TcSmem<NB, GPT>;
+  constexpr int READERS = NB == 64 && GPT == 1 ? 8 : 16, SETS = (kTcCopyCodes - READERS) / 4;
   extern __shared__ unsigned char tc_raw[];
   unsigned char *smem =
       reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~(uintptr_t)1023);
@@ -178,8 +192,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   auto scales = [&](int i, int g) { return reinterpret_cast<float *>(smem + L::kScales) + (i * GPT + g) * kTcRows; };
   uint64_t *x_full = reinterpret_cast<uint64_t *>(smem + L::kBars), *a_full = x_full + kTcRing,
            *done = a_full + kTcRing, *c_full = done + kTcRing, *c_empty = c_full + kTcCodeRing,
-           *d_full = c_empty + kTcCodeRing, *d_empty = d_full + kTcD;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_empty + kTcD);
+           *d_full = c_empty + kTcCodeRing, *d_empty = d_full + L::kD;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_empty + L::kD);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)blockIdx.x % cs, item0 = (int)blockIdx.x / cs, istep = (int)gridDim.x / cs;
@@ -190,9 +204,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // done: a tile's MMAs, which leave the places of its x and its unpacked codes free
     for (int i = 0; i < kTcRing; ++i)
       mbar_init(smem_addr(&x_full[i]), 1), mbar_init(smem_addr(&a_full[i]), 4),
-          mbar_init(smem_addr(&done[i]), GPT == 1 ? 1 : kTcD);
+          mbar_init(smem_addr(&done[i]), GPT == 1 ? 1 : kTcMmas);
     for (int i = 0; i < kTcCodeRing; ++i) mbar_init(smem_addr(&c_full[i]), 1), mbar_init(smem_addr(&c_empty[i]), 4);
-    for (int i = 0; i < kTcD; ++i) mbar_init(smem_addr(&d_full[i]), 1), mbar_init(smem_addr(&d_empty[i]), kTcReaders);
+    for (int i = 0; i < L::kD; ++i) mbar_init(smem_addr(&d_full[i]), 1), mbar_init(smem_addr(&d_empty[i]), READERS);
     mbar_init_fence();
   }
   if (warp == kTcMma) {
@@ -210,11 +224,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   pdl_wait();  // x is the preceding kernel's output, and the weight may be too
   pdl_trigger();
 
-  if (warp < kTcReaders) {
+  if (warp < READERS) {
     // read D, scale, sum: batch rows c0 .. + COLS of the item
-    constexpr int COLS = NB * 4 / kTcReaders;
+    constexpr int COLS = NB * 4 / READERS;
     const int c0 = warp / 4 * COLS, lrow = tid % 128;
-    TcPos<kTcD> d;
+    TcPos<L::kD> d;
     bool live = true;
     int tile = 0;
     for (int item = item0; item < items; item += istep) {
@@ -224,7 +238,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int m = 0; m < COLS; ++m) acc[m] = 0.f;
       for (int g = 0; g < (k1 - k0) * GPT; ++g) {
         if (live) live = tc_wait(smem_addr(&d_full[d.s]), d.ph);
-        const float s = scales(tile & (kTcScaleRing - 1), GPT == 1 ? 0 : g & (GPT - 1))[lrow];
+        const float s = scales(tile & (L::kScaleRing - 1), GPT == 1 ? 0 : g & (GPT - 1))[lrow];
         if (GPT == 1 || (g & (GPT - 1)) == GPT - 1) ++tile;
         __syncwarp();
         tc_after();
@@ -265,70 +279,76 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else if (warp < kTcCopyCodes) {
     // unpack: this warp's rows of every other tile, and their scales
-    const int quarter = warp & 3, set = (warp - kTcReaders) >> 2, lrow = quarter * 32 + lane;
-    TcPos<kTcCodeRing> c;
-    TcPos<kTcRing> a;
-    bool live = true;
-    int i = 0;
-    for (int item = item0; item < items; item += istep) {
+    const int quarter = warp & 3, set = (warp - READERS) >> 2, lrow = quarter * 32 + lane;
+    const int per = k1 - k0, total = item0 < items ? (items - item0 + istep - 1) / istep * per : 0;
+    uint32_t zraw[GPT], sraw[GPT];  // zeros and scales of this warp's next tile, as they lie in memory
+    int next = set, item = item0, kt = k0 + set;
+    // a tile's loads are asked for before the tile before it is unpacked, also
+    // from one item to the next
+    auto fetch = [&] {
+      if (next >= total) return;
+      while (kt >= k1) kt -= per, item += istep;
       const int64_t n = min(item / p.mtiles * kTcRows + lrow, p.N - 1);
-      const uint8_t *zrow = p.zeros ? p.zeros + n * p.z_ld : nullptr;
       const int64_t srow = n * p.s_ld;
-      uint32_t zraw[GPT], sraw[GPT];  // zeros and scales of this warp's next tile, as they lie in memory
-      auto fetch = [&](int kt) {
+      const uint8_t *zrow = p.zeros ? p.zeros + n * p.z_ld : nullptr;
 #pragma unroll
-        for (int j = 0; j < GPT; ++j) {
-          const int g = min(kt * GPT + j, p.groups - 1);
-          zraw[j] = zrow ? zrow[g] : 8u;
+      for (int j = 0; j < GPT; ++j) {
+        const int g = kt * GPT + j;
+        zraw[j] = 8u, sraw[j] = 0u;  // of a group wholly past K, whose sum is 0
+        if (g < p.groups) {
+          if (zrow) zraw[j] = zrow[g];
           sraw[j] = p.s_bf16 ? (uint32_t) static_cast<const uint16_t *>(p.scales)[srow + g]
                              : static_cast<const uint32_t *>(p.scales)[srow + g];
         }
-      };
-      fetch(k0 + ((i & 1) != set));
-      for (int kt = k0; kt < k1; ++kt, ++i, c.next(), a.next()) {
-        if ((i & 1) != set) continue;
-        uint32_t zz[GPT];  // (128 + z, 128 + z)
-        float sc[GPT];     // of a group wholly past K, whose sum is 0, 0
+      }
+      next += SETS, kt += SETS;
+    };
+    bool live = true;
+    fetch();
+    for (int i = set; i < total; i += SETS) {
+      const int c = i % kTcCodeRing, a = i % kTcRing;
+      uint32_t zz[GPT];  // (128 + z, 128 + z)
+      float sc[GPT];
 #pragma unroll
-        for (int j = 0; j < GPT; ++j) {
-          zz[j] = 0x43004300u + zraw[j] * 0x10001u;
-          sc[j] = kt * GPT + j < p.groups ? __uint_as_float(p.s_bf16 ? sraw[j] << 16 : sraw[j]) : 0.f;
+      for (int j = 0; j < GPT; ++j) {
+        zz[j] = 0x43004300u + zraw[j] * 0x10001u;
+        sc[j] = __uint_as_float(p.s_bf16 ? sraw[j] << 16 : sraw[j]);
+      }
+      fetch();
+      if (live) live = tc_wait(smem_addr(&c_full[c]), i / kTcCodeRing & 1);
+      const uint4 *src = reinterpret_cast<const uint4 *>(codes(c)) + lrow * 4;
+      uint4 q[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) q[t] = src[t];
+      if (live) live = tc_wait(smem_addr(&done[a]), (i / kTcRing & 1) ^ 1);
+      // tile i - 4 is done, so its accumulator's tile before, i - 4 - kD or a
+      // later one, has been read, and the scales of all up to that
+#pragma unroll
+      for (int j = 0; j < GPT; ++j) scales(i & (L::kScaleRing - 1), j)[lrow] = sc[j];
+      __syncwarp();
+      tc_after();
+      const uint32_t at = tmem + (uint32_t)(a * 64) + ((uint32_t)(32 * quarter) << 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // columns 32 j ..: words 4 t + j
+        uint32_t r[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t w = j == 0 ? q[t].x : j == 1 ? q[t].y : j == 2 ? q[t].z : q[t].w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[4 * t + e] = w4_pair(w, e, zz[j * GPT / 4], p.mask, p.magic);
         }
-        fetch(kt + 2);
-        if (live) live = tc_wait(smem_addr(&c_full[c.s]), c.ph);
-        const uint4 *src = reinterpret_cast<const uint4 *>(codes(c.s)) + lrow * 4;
-        uint4 q[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) q[t] = src[t];
-        if (live) live = tc_wait(smem_addr(&done[a.s]), a.ph ^ 1u);
-        // the tile 4 before is done, so that of 6 before has been read, and its scales with it
-#pragma unroll
-        for (int j = 0; j < GPT; ++j) scales(i & (kTcScaleRing - 1), j)[lrow] = sc[j];
-        __syncwarp();
-        tc_after();
-        const uint32_t at = tmem + (uint32_t)(a.s * 64) + ((uint32_t)(32 * quarter) << 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // columns 32 j ..: words 4 t + j
-          uint32_t r[16];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint32_t w = j == 0 ? q[t].x : j == 1 ? q[t].y : j == 2 ? q[t].z : q[t].w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[4 * t + e] = w4_pair(w, e, zz[j * GPT / 4], p.mask, p.magic);
-          }
-          tc_st16(at + 16 * j, r);
-        }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc_before();
-        __syncwarp();
-        if (lane == 0) {
-          tc_arrive(smem_addr(&a_full[a.s]));
-          tc_arrive(smem_addr(&c_empty[c.s]));  // here, where the codes have been used: an arrival may overtake a load
-        }
+        tc_st16(at + 16 * j, r);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_before();
+      __syncwarp();
+      if (lane == 0) {
+        tc_arrive(smem_addr(&a_full[a]));
+        tc_arrive(smem_addr(&c_empty[c]));  // here, where the codes have been used: an arrival may overtake a load
       }
     }
   } else if (warp == kTcCopyCodes) {
-    if (lane == 0) {
+    if (tc_elect()) {
       TcPos<kTcCodeRing> c;
       int issued = 0;
       bool live = true;
@@ -349,7 +369,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     __syncwarp();
   } else if (warp == kTcCopyX) {
-    if (lane == 0) {
+    if (tc_elect()) {
       TcPos<kTcRing> c;
       int issued = 0;
       bool live = true;
@@ -370,14 +390,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     __syncwarp();
   } else {
-    if (lane == 0) {
+    if (tc_elect()) {
       // fp32 accumulator, bf16 A and B, both K-major, N / 8 and M / 16
       const uint32_t idesc =
           (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NB >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
-      const int me = warp - kTcMma;  // its accumulator: that of every other group
-      const uint32_t acc = tmem_d + (uint32_t)(me * NB);
+      // every other group, the accumulators in turn
+      const int me = warp - kTcMma;
       TcPos<kTcRing> c, last;
-      uint32_t dph = 1u;
+      TcPos<L::kD / kTcMmas> d;
       bool live = true, any = false;
       int i = 0;
       for (int item = item0; item < items && live; item += istep) {
@@ -386,16 +406,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           live = tc_wait(smem_addr(&x_full[c.s]), c.ph) && tc_wait(smem_addr(&a_full[c.s]), c.ph);
           if (!live) break;
           const uint32_t ta = tmem + (uint32_t)(c.s * 64), sb = smem_addr(xs(c.s));
-          for (int g = GPT == 1 ? 0 : me; g < GPT; g += kTcD) {
-            if (live) live = tc_wait(smem_addr(&d_empty[me]), dph);
-            dph ^= 1u;
+          for (int g = GPT == 1 ? 0 : me; g < GPT; g += kTcMmas, d.next()) {
+            const int at = me + kTcMmas * d.s;
+            if (live) live = tc_wait(smem_addr(&d_empty[at]), d.ph ^ 1u);
             tc_after();
 #pragma unroll
             for (int j = 0; j < 8 / GPT; ++j) {
               const int step = g * (8 / GPT) + j;  // 16 columns
-              tc_mma(acc, ta + 8 * step, tc_desc(sb + (step >> 2) * (L::kX / 2) + (step & 3) * 32), idesc, j != 0);
+              tc_mma(tmem_d + (uint32_t)(at * NB), ta + 8 * step,
+                     tc_desc(sb + (step >> 2) * (L::kX / 2) + (step & 3) * 32), idesc, j != 0);
             }
-            tc_commit(smem_addr(&d_full[me]));
+            tc_commit(smem_addr(&d_full[at]));
           }
           tc_commit(smem_addr(&done[c.s]));
           last = c, any = true;
@@ -451,7 +472,7 @@ cudaError_t launch_tc_t(W4Params p, cudaStream_t stream, bool *taken) {
   *taken = true;
   const int items = (int)all, sms = sm_count_current();
   int cs = 1;
-  while (cs < 4 && items * cs * 2 <= sms && cs * 4 <= p.tiles) cs *= 2;
+  while (p.tiles >= 12 && cs < 4 && items * cs * 2 <= sms) cs *= 2;
   const int grid = cs > 1 ? items * cs : min(items, sms);
   auto kern = w4_tc_kernel<NB, GPT>;
   static LaunchCache cache;

@@ -189,7 +189,7 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
 
     x is fp32 or bf16 with any row stride; the output has ``out_dtype`` (x's
     type by default).  Written for the batches of a decode step, right for
-    any M.  The codes' products with x must stay within fp32's range before
+    any M; from about 256 rows on the product with a bf16 weight is faster.  The codes' products with x must stay within fp32's range before
     the scale; codes, scales and zeros take less than 4 GB each.  Inference
     only: x or scales with a gradient are refused."""
     global _host
