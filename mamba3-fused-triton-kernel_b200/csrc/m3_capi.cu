@@ -448,6 +448,8 @@ int m3_siso_step(const m3_dims *dims, const m3_step_args *args, m3_stream_t stre
 }
 
 int m3_device_error(int reset) {
+  // the copies below wait for blocking streams only
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
   const int a = m3::siso_device_error(reset != 0);
   const int b = m3::mimo_device_error(reset != 0);
   const int c = m3::step_device_error(reset != 0);
