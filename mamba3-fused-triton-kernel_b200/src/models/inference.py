@@ -48,6 +48,8 @@ this package.  Differences from the reference, all deliberate:
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 import torch.nn.functional as F
 
@@ -94,6 +96,27 @@ def single_launch_preferred(model, batch: int, graph: bool = False) -> bool:
     return batch <= SINGLE_LAUNCH_MAX_BATCH and flop <= limit
 from src.kernels.utils import apply_rope
 from src.models.mamba3 import Mamba3
+
+
+def check_device_error(layers) -> None:
+    """``Mamba3Decoder.check_device_error`` for the layers of one decoder:
+    one read of their device's word, the step workspaces of all of them
+    zeroed."""
+    device = layers[0].model.in_proj.weight.device
+    with _native.device_guard(device) if device.type == "cuda" else contextlib.nullcontext():
+        err = _native.device_error(reset=True)
+    if err == 0:
+        return
+    for layer in layers:
+        launch = layer._step_cache[1] if layer._step_cache is not None else None
+        if launch is not None:
+            launch.workspace.zero_()
+            torch.cuda.synchronize(launch.workspace.device)
+    if err < 0:
+        raise RuntimeError("the library's device error word could not be read")
+    raise RuntimeError(f"a decode kernel gave up a bounded wait (device error {err:#x}): the outputs "
+                       "and state of the steps since the last check are undefined; the step "
+                       "workspace has been zeroed again")
 
 
 class Mamba3Decoder:
@@ -255,18 +278,7 @@ class Mamba3Decoder:
         caller has restored a state it trusts.  Synchronises the device.
         Called by ``warmup_cuda_graph``, every ``DEVICE_ERROR_INTERVAL``
         calls of ``step_host`` and at the end of ``decode_sequence``."""
-        err = _native.device_error(reset=True)
-        if err == 0:
-            return
-        launch = self._step_cache[1] if self._step_cache is not None else None
-        if launch is not None:
-            launch.workspace.zero_()
-            torch.cuda.synchronize(launch.workspace.device)
-        if err < 0:
-            raise RuntimeError("the library's device error word could not be read")
-        raise RuntimeError(f"a decode kernel gave up a bounded wait (device error {err:#x}): the outputs "
-                           "and state of the steps since the last check are undefined; the step "
-                           "workspace has been zeroed again")
+        check_device_error((self,))
 
     def step(self, u: torch.Tensor, state: dict) -> tuple:
         """One decode step: u (batch, d_model) -> (out (batch, d_model), state)."""

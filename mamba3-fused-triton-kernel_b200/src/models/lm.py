@@ -36,7 +36,7 @@ from src.kernels.linear import linear
 from src.kernels.linear_w4 import W4Projection
 from src.kernels.logits import next_tokens
 from src.kernels.norm import residual_rmsnorm
-from src.models.inference import Mamba3Decoder
+from src.models.inference import Mamba3Decoder, check_device_error
 
 
 class Mamba3LMDecoder:
@@ -115,10 +115,19 @@ class Mamba3LMDecoder:
         for _ in range(n_warmup):
             self._step_eager(self._graph_ids, states)
         torch.cuda.synchronize(h.device)
+        self.check_device_error()
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):
             self._graph_logits = self._step_eager(self._graph_ids, states)
+
+    def check_device_error(self) -> None:
+        """Raise if a library kernel gave up a bounded wait since the last
+        check; logits, tokens and states since then are undefined
+        (``Mamba3Decoder.check_device_error``).  Synchronises the device.
+        Called by ``warmup_cuda_graph`` and at the end of ``decode_sequence``
+        (not while it is captured) and ``generate``."""
+        check_device_error(self.layers)
 
     def step(self, input_ids: torch.Tensor, states: list) -> tuple:
         """One token per sequence: ``input_ids`` (batch,) -> (logits
@@ -143,6 +152,8 @@ class Mamba3LMDecoder:
             for t in range(L):
                 logits, states = self.step(input_ids[:, t], states)
                 outs.append(logits.clone())
+        if self.cuda and L > 0 and not (input_ids.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self.check_device_error()
         return torch.stack(outs, dim=1), states
 
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, *, prompt_lengths: torch.Tensor | None = None,
@@ -166,7 +177,8 @@ class Mamba3LMDecoder:
         ``lengths`` counts a row's prompt and what it produced (its
         ``eos_token_id`` with it); places behind that hold 0, as do the
         logprobs of the prompt.  Only the model's own vocabulary is produced,
-        not what pads it.  Needs a CUDA backend."""
+        not what pads it.  Waits for the GPU once at the end, to raise if a
+        kernel gave up (``check_device_error``).  Needs a CUDA backend."""
         if not self.cuda:
             raise RuntimeError("generate needs a CUDA backend")
         assert input_ids.is_cuda and input_ids.dim() == 2 and input_ids.shape[1] > 0, \
@@ -222,4 +234,5 @@ class Mamba3LMDecoder:
                 lengths += write
                 if eos_token_id is not None:
                     going &= ~(write & (ids == eos_token_id))
+        self.check_device_error()
         return tokens, logprobs, lengths

@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from src.kernels.norm import residual_rmsnorm
-from src.models.inference import Mamba3Decoder
+from src.models.inference import Mamba3Decoder, check_device_error
 
 
 class Mamba3StackDecoder:
@@ -77,6 +77,7 @@ class Mamba3StackDecoder:
         for _ in range(n_warmup):
             self._step_eager(self._graph_input, states)
         torch.cuda.synchronize(h.device)
+        check_device_error(self.layers)
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):
