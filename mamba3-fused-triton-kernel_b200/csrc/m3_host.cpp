@@ -33,6 +33,11 @@ int dtype_code(at::ScalarType t) { return t == at::kFloat ? M3_F32 : t == at::kB
 
 bool on(const at::Tensor &t, int dev) { return t.is_cuda() && t.get_device() == dev; }
 
+// it asks for a gradient, also a forward-mode one: the Python path refuses it
+bool wants_gradient(const at::Tensor &t) {
+  return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 m3_stream_t stream_of(int dev) {
   return reinterpret_cast<m3_stream_t>(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream());
 }
@@ -52,7 +57,7 @@ PyObject *linear_w4(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const int dev = x.get_device(), xd = dtype_code(x.scalar_type()), sd = dtype_code(scales.scalar_type());
   const int64_t M = x.size(0), K = x.size(1), N = scales.size(0), groups = scales.size(1);
   if (xd < 0 || sd < 0 || M <= 0 || K <= 0 || N <= 0 || M > INT32_MAX || K > INT32_MAX || N > INT32_MAX ||
-      !x.is_contiguous() || ((x.requires_grad() || scales.requires_grad()) && at::GradMode::is_enabled()) ||
+      !x.is_contiguous() || wants_gradient(x) || wants_gradient(scales) ||
       codes.scalar_type() != at::kInt || !codes.is_contiguous() || codes.size(0) != (N + 15) / 16 ||
       codes.size(1) != (K + 127) / 128 || codes.size(2) != 16 || codes.size(3) != 16 ||
       groups != (K + group - 1) / group || !scales.is_contiguous() || !on(codes, dev) || !on(scales, dev) ||
@@ -89,7 +94,8 @@ bool per_row(PyObject *o, int64_t B, int dev, const float **ptr, float *value, f
   }
   if (!is_tensor(o)) return false;
   const at::Tensor &t = tensor(o);
-  if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != B || !t.is_contiguous() || !on(t, dev))
+  if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != B || !t.is_contiguous() || !on(t, dev) ||
+      wants_gradient(t))
     return false;
   *ptr = static_cast<const float *>(t.data_ptr());
   return true;
@@ -116,7 +122,7 @@ bool shared_rows(PyObject *o, at::ScalarType dt, int64_t B, int64_t width, int d
   const at::Tensor &t = tensor(o);
   const int64_t d = t.dim();
   if (t.scalar_type() != dt || (d != 1 && d != 2) || t.size(d - 1) < width || t.stride(d - 1) != 1 ||
-      (d == 2 && t.size(0) != B) || !on(t, dev) || (t.requires_grad() && at::GradMode::is_enabled()))
+      (d == 2 && t.size(0) != B) || !on(t, dev) || wants_gradient(t))
     return false;
   *ptr = t.data_ptr(), *stride = d == 2 && B > 1 ? t.stride(0) : 0;
   return true;
@@ -131,7 +137,7 @@ bool adjust_args(PyObject *const *a, m3_logits_args *g, int *dev_out) {
   const int64_t B = logits.size(0), V = logits.size(1);
   g->dtype = dtype_code(logits.scalar_type());
   if (g->dtype < 0 || B <= 0 || V <= 0 || B > INT32_MAX || V > (1 << 30) || logits.stride(1) != 1 ||
-      (logits.requires_grad() && at::GradMode::is_enabled()) || c10::cuda::current_device() != dev)
+      wants_gradient(logits) || c10::cuda::current_device() != dev)
     return false;
   g->B = (int32_t)B, g->V = (int32_t)V, g->logits = logits.data_ptr(), g->ld = logits.stride(0);
   if (a[1] != Py_None) {

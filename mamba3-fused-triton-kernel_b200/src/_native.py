@@ -23,6 +23,7 @@ import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "lib", "libmamba3_b200.so")
@@ -204,6 +205,16 @@ def require_cuda_available(what: str = "the CUDA decode backend") -> None:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def wants_gradient(*tensors) -> bool:
+    """Whether one of the tensors (None among them) asks its results for a
+    gradient: it requires one with gradients enabled, or has a forward-mode
+    tangent."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(
+        t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 HOST_PATH = os.path.join(os.path.dirname(LIB_PATH), "m3_host.so")

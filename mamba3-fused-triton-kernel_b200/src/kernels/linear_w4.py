@@ -191,7 +191,8 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     type by default).  Written for the batches of a decode step, right for
     any M; from about 256 rows on the product with a bf16 weight is faster.  The codes' products with x must stay within fp32's range before
     the scale; codes, scales and zeros take less than 4 GB each.  Inference
-    only: x or scales with a gradient are refused."""
+    only: x or scales that ask for a gradient, also a forward-mode one, are
+    refused."""
     global _host
     if out_dtype is None:
         if _host is None:
@@ -203,7 +204,7 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
         _check_group(group_size)
     dev = x.get_device() if x.is_cuda else -1
     assert dev >= 0 and x.dim() == 2, "x must be a (M, K) CUDA tensor"
-    if (x.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
+    if nat.wants_gradient(x, scales):
         raise RuntimeError("linear_w4 has no gradient: call it under torch.no_grad() or on detached tensors")
     M, K = x.shape
     N, groups = scales.shape

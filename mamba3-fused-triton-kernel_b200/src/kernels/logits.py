@@ -69,6 +69,11 @@ def _shared_rows(name: str, value: torch.Tensor, dtype: torch.dtype, B: int, wid
     return value.data_ptr(), value.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
 
 
+def _refuse_gradients(*values) -> None:
+    if nat.wants_gradient(*(v for v in values if isinstance(v, torch.Tensor))):
+        raise RuntimeError("the logit operators have no gradient: call them under torch.no_grad() or detach")
+
+
 def _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
                  bias, allowed, keep: list) -> tuple:
     """Checked arguments that both entry points share: the packed fields up
@@ -78,8 +83,7 @@ def _adjust_args(logits, tokens, lengths, prompt_lengths, repetition_penalty, pr
     B, V = logits.shape
     code = _CODE.get(logits.dtype)
     assert code is not None, f"logits must be float32 or bfloat16 (got {logits.dtype})"
-    if (logits.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
-        raise RuntimeError("the logit operators have no gradient: call them under torch.no_grad() or detach")
+    _refuse_gradients(logits, bias, repetition_penalty, presence_penalty, frequency_penalty)
     if logits.is_contiguous():
         ld = V
     else:
@@ -152,8 +156,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             the logits' type without it.
 
     Penalties given as tensors are not looked at by the host: a repetition
-    penalty is above 0.  Inference only: logits or a bias with a gradient are
-    refused."""
+    penalty is above 0.  Inference only: logits, a bias or penalties that ask
+    for a gradient, also a forward-mode one, are refused."""
     global _host_process
     if out is None:
         if _host_process is None:
@@ -236,6 +240,7 @@ def next_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     seed_ptr = pos_ptr = 0
     if temperature is not None:
         sample = 1
+        _refuse_gradients(temperature)
         temp, temp_value = _per_row("temperature", temperature, 0.0, B, dev, keep)
         assert seeds is not None, "a temperature needs seeds"
         assert seeds.dtype == torch.int64 and (positions is None or positions.dtype == torch.int64), \
