@@ -191,6 +191,9 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two (B, V) tensors may share memory.  Rows at the same
+    distance are told apart (parts of the columns of one buffer); others go
+    by their first and last bytes."""
     def span(t):
         if t.numel() == 0:
             return 0, 0
@@ -198,7 +201,14 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if not (a0 < b1 and b0 < a1):
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if a.shape[0] == 1 or pitch == 0 or pitch != b.stride(0) * b.element_size() or \
+            (a.shape[1] > 1 and (a.stride(1) != 1 or b.stride(1) != 1)):
+        return True
+    at = (b0 - a0) % pitch  # b's rows from a's
+    return at < a.shape[1] * a.element_size() or at + b.shape[1] * b.element_size() > pitch
 
 
 def next_tokens(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
