@@ -208,6 +208,10 @@ class Mamba3LMDecoder:
             raise ValueError(f"prompt_lengths must be in [1, {L}]")
         if eos_token_id is not None and not 0 <= eos_token_id < vocab:
             raise ValueError(f"eos_token_id must be in [0, {vocab})")
+        assert temperature is None or seeds is not None, "a temperature needs seeds"
+        given = states if states is not None else self._graph_states
+        if given is not None and given[0]["ssm_state"].shape[0] != B:
+            raise ValueError(f"the states hold {given[0]['ssm_state'].shape[0]} rows, input_ids {B}")
         if states is None:
             if self._graph is not None:
                 states = self._graph_states
