@@ -144,15 +144,18 @@ class W4Projection:
     same tensors, once the weight has been replaced or modified in place.  A
     change that PyTorch does not count (through ``.data``) needs
     ``refresh()``.  A captured graph replays what the tensors hold: it sees a
-    change after the next ``get()``.  Quantising waits for the GPU: it belongs
-    before a capture."""
+    change after the next ``get()``.  A weight of another shape, type or
+    device gets new tensors; the old ones are kept, since a captured graph
+    may still read them, and such a graph does not see the change.  Quantising
+    waits for the GPU: it belongs before a capture."""
 
-    __slots__ = ("weight", "group_size", "source", "key", "w4")
+    __slots__ = ("weight", "group_size", "source", "key", "w4", "kept")
 
     def __init__(self, weight, group_size: int):
         _check_group(group_size)
         self.weight, self.group_size = weight, group_size  # weight: a callable, the current parameter
         self.source = self.key = self.w4 = None
+        self.kept = []
         self.get()
 
     def get(self) -> W4Weight:
@@ -173,6 +176,8 @@ class W4Projection:
             old.codes.copy_(new.codes)
             old.scales.copy_(new.scales)
         else:
+            if old is not None:
+                self.kept.append(old)
             self.w4 = new
         self.source, self.key = w, (w._version, w.data_ptr(), w.dtype)
 
