@@ -201,6 +201,7 @@ class Mamba3Decoder:
             step_fn(self._graph_input, state)
         torch.cuda.synchronize(device)
         self.check_device_error()
+        self._update_w4()
         self._cuda_graph = torch.cuda.CUDAGraph()
         self._host_graph = None
         self._host_output = None
@@ -361,6 +362,11 @@ class Mamba3Decoder:
         """The weight a projection of the full-fused backend uses: the
         model's, or its 4-bit form."""
         return getattr(self.model, name).weight if self._w4 is None else self._w4[name].get()
+
+    def _update_w4(self) -> None:
+        """Quantise what has changed now: it cannot be done in a capture."""
+        for projection in (self._w4 or {}).values():
+            projection.get()
 
     def _single_launch(self, state: dict, graph: bool = False):
         """Prepared single-launch step for this state and the current

@@ -116,6 +116,10 @@ class Mamba3LMDecoder:
             self._step_eager(self._graph_ids, states)
         torch.cuda.synchronize(h.device)
         self.check_device_error()
+        for layer in self.layers:
+            layer._update_w4()
+        for projection in (self._w4 or {}).values():
+            projection.get()
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):

@@ -78,6 +78,8 @@ class Mamba3StackDecoder:
             self._step_eager(self._graph_input, states)
         torch.cuda.synchronize(h.device)
         check_device_error(self.layers)
+        for layer in self.layers:
+            layer._update_w4()
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):
