@@ -9,7 +9,7 @@ statically, so the library only needs the driver at run time.  Objects go to
 ``csrc/`` / the repository ``include/`` is newer than its object.  Also builds
 ``lib/m3_host.so`` from ``csrc/m3_host.cpp`` (a Python module on PyTorch's C++
 interface, no CUDA code): the host-side fast path of the language-model
-operators.
+operators, left out where PyTorch or g++ is missing.
 """
 
 from __future__ import annotations
@@ -93,26 +93,40 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int = 0) -> st
     return LIB
 
 
-def build_host(nvcc: str, force: bool = False) -> None:
+def build_host(nvcc: str, force: bool = False) -> bool:
     """``lib/m3_host.so``, with the C++ compiler and the headers of the
-    PyTorch that this interpreter imports."""
+    PyTorch that this interpreter imports.  Where one of them is missing it
+    is left out with a warning: the operators then take the Python path.
+    True if the module stands."""
     newest = max(os.path.getmtime(HOST_SRC), *(os.path.getmtime(h) for h in glob.glob(os.path.join(INCLUDE, "*.h"))))
     if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= newest:
-        return
-    import torch
+        return True
+    try:
+        import torch
+        base = os.path.dirname(torch.__file__)
+    except ImportError:
+        base = None
+    cxx = shutil.which("g++")
+    missing = "PyTorch" if base is None else "g++" if cxx is None else \
+        None if os.path.exists(os.path.join(base, "include", "torch", "csrc", "Exceptions.h")) else "PyTorch's headers"
+    if missing is not None:
+        if os.path.exists(HOST_LIB):
+            os.remove(HOST_LIB)  # of other sources than the library
+        print(f"warning: {missing} not found, {os.path.basename(HOST_LIB)} is left out", file=sys.stderr)
+        return False
 
-    base = os.path.dirname(torch.__file__)
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include"), INCLUDE]
     libs = os.path.join(base, "lib")
     tmp = HOST_LIB + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + i for i in inc), HOST_SRC,
            "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST_LIB)
+    return True
 
 
 def main():
