@@ -32,6 +32,7 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmamba3_b200.so")
 HOST_SRC = os.path.join(CSRC, "m3_host.cpp")
 HOST_LIB = os.path.join(LIBDIR, "m3_host.so")
+HOST_STAMP = os.path.join(BUILD, "m3_host.torch")  # the PyTorch it was built with
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3",
@@ -95,23 +96,25 @@ def build(force: bool = False, ptxas_verbose: bool = False, jobs: int = 0) -> st
 
 def build_host(nvcc: str, force: bool = False) -> bool:
     """``lib/m3_host.so``, with the C++ compiler and the headers of the
-    PyTorch that this interpreter imports.  Where one of them is missing it
-    is left out with a warning: the operators then take the Python path.
-    True if the module stands."""
-    newest = max(os.path.getmtime(HOST_SRC), *(os.path.getmtime(h) for h in glob.glob(os.path.join(INCLUDE, "*.h"))))
-    if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= newest:
-        return True
+    PyTorch that this interpreter imports; rebuilt for another PyTorch, whose
+    objects may be laid out differently.  Where one of them is missing it is
+    left out with a warning: the operators then take the Python path.  True
+    if the module stands."""
     try:
         import torch
-        base = os.path.dirname(torch.__file__)
+        base, version = os.path.dirname(torch.__file__), str(torch.__version__)
     except ImportError:
-        base = None
+        base = version = None
+    newest = max(os.path.getmtime(HOST_SRC), *(os.path.getmtime(h) for h in glob.glob(os.path.join(INCLUDE, "*.h"))))
+    if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= newest and \
+            version is not None and _host_version() == version:
+        return True
     cxx = shutil.which("g++")
     missing = "PyTorch" if base is None else "g++" if cxx is None else \
         None if os.path.exists(os.path.join(base, "include", "torch", "csrc", "Exceptions.h")) else "PyTorch's headers"
     if missing is not None:
         if os.path.exists(HOST_LIB):
-            os.remove(HOST_LIB)  # of other sources than the library
+            os.remove(HOST_LIB)  # of other sources than the library, or for another PyTorch
         print(f"warning: {missing} not found, {os.path.basename(HOST_LIB)} is left out", file=sys.stderr)
         return False
 
@@ -120,13 +123,24 @@ def build_host(nvcc: str, force: bool = False) -> bool:
     libs = os.path.join(base, "lib")
     tmp = HOST_LIB + ".tmp"
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + i for i in inc), HOST_SRC,
+           f'-DM3_TORCH_VERSION="{version}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + i for i in inc), HOST_SRC,
            "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST_LIB)
+    with open(HOST_STAMP, "w") as f:
+        f.write(version)
     return True
+
+
+def _host_version() -> str | None:
+    """The PyTorch that the module was built with."""
+    try:
+        with open(HOST_STAMP) as f:
+            return f.read()
+    except OSError:
+        return None
 
 
 def main():

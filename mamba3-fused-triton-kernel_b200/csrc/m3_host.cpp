@@ -238,4 +238,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "m3_host", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_m3_host() { return PyModule_Create(&module); }
+// torch_version: the PyTorch whose object layouts are compiled in here
+PyMODINIT_FUNC PyInit_m3_host() {
+  PyObject *m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", M3_TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -226,6 +226,15 @@ def _no_host(*args):
     return None
 
 
+def _check_host(module) -> None:
+    """ImportError unless the host module was built with this PyTorch: it has
+    the layouts of its objects compiled in, which resolved symbols do not
+    show."""
+    built = getattr(module, "torch_version", None)
+    if built != str(torch.__version__):
+        raise ImportError(f"it was built with {built or 'an unnamed one'}, this is {torch.__version__}")
+
+
 def host_entry(name: str):
     """The host module's function ``name`` (csrc/m3_host.cpp): called with an
     operator's positional arguments it returns the result, or None for a call
@@ -240,6 +249,7 @@ def host_entry(name: str):
         try:
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
+            _check_host(module)
         except ImportError as e:
             raise RuntimeError(f"{HOST_PATH} does not fit this PyTorch ({e}); run "
                                "`python mamba3-fused-triton-kernel_b200/build_native.py --force`") from e
