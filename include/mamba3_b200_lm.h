@@ -39,9 +39,10 @@ extern "C" {
  *   group   32, 64 or 128
  * Codes, scales and zeros take less than 4 GB each (M3_ERR_SHAPE).
  * Products are exact (a bf16 x times a small integer; an fp32 x is taken as
- * three bf16 terms), sums are fp32, scaled once per group and added in a
- * fixed order: the same call gives the same bits.  The sum of a group before
- * its scale has to stay within fp32's range. */
+ * three bf16 terms, which are all of it from 2^-110 on, and to less than
+ * 2^-133 below), sums are fp32, scaled once per group and added in a fixed
+ * order: the same call gives the same bits.  The sum of a group before its
+ * scale has to stay within fp32's range. */
 typedef struct m3_w4_args {
   int32_t M, N, K, group;
   const void *x;      int64_t ldx;          int32_t x_dtype;

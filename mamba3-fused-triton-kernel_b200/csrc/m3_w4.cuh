@@ -40,8 +40,10 @@ __device__ __forceinline__ uint32_t w4_pair(uint32_t w, int i, uint32_t zz, uint
 }
 
 // 8 consecutive elements of a batch row as bf16 terms: one for bf16 x, three
-// for fp32 x (head, middle, rest; each the truncation of what is left, so
-// that head + middle + rest is x).  An infinite x is its head alone.
+// for fp32 x (head, middle, rest; each the truncation of what is left).  The
+// 24 bits of an x of 2^-110 or more end at or above bf16's smallest subnormal
+// number, 2^-133, so head + middle + rest is x; of a smaller x what lies below
+// that is dropped.  An infinite x is its head alone.
 template <typename XT>
 struct W4X;
 
