@@ -422,8 +422,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           last = c, any = true;
         }
       }
-      // the commits' arrivals land before this thread leaves
-      if (any && live) tc_wait(smem_addr(&done[last.s]), last.ph);
+      // the MMAs issued end, and the commits' arrivals land, before this thread
+      // leaves and the tensor memory is freed, also behind a wait that ran out
+      if (any) tc_wait(smem_addr(&done[last.s]), last.ph);
     }
     __syncwarp();
   }
