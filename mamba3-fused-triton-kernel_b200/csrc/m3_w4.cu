@@ -462,7 +462,9 @@ template <typename XT, int GPT, bool ZEROS>
 cudaError_t launch_w4_x(const W4Params &p, cudaStream_t stream) {
   bool taken = false;
   cudaError_t e = cudaSuccess;
-  // the largest batch tile whose x fits in shared memory
+  // the largest batch tile whose x fits in shared memory, whatever M: fp32 rows
+  // of 2,048 x 4,096, where that is 8, here / in the direct kernel, us: 64 rows
+  // 18 / 112, 256 rows 55 / 183, 4,096 rows 795 / 2,091
   if (p.M > 16) e = launch_w4_stream<XT, 4, 1, GPT, ZEROS>(p, stream, &taken);
   if (!taken && e == cudaSuccess && p.M > 8) {
     if constexpr (GPT != 4)
@@ -508,7 +510,11 @@ cudaError_t launch_linear_w4(const m3_w4_args &a, cudaStream_t stream) {
   // 8.8 / 8.8; 4,224 x 1,024 (14.3), 64 rows 7.3 / 5.7, 128 rows 8.8 / 8.4.  17
   // to 32 rows take more work, and groups of 128, whose sums are read back
   // least often: 32 rows of 50,280 x 2,560 31 / 42, of 9,440 x 2,048 11.0 / 9.3;
-  // with groups of 64 48 / 44.
+  // with groups of 64 48 / 44.  Finer groups at 64 rows, G 64 and G 32: 50,280 x
+  // 2,560 48 / 77 and 74 / 93, 20,000 x 1,024 (67.6) 15.3 / 23.3 and 22.3 / 26.1,
+  // 9,440 x 2,048 (63.8) 12.9 / 14.7 and 17.1 / 17.6, 4,096 x 2,048 9.4 / 9.3 and
+  // 11.9 / 10.8: for groups of 32 the two cross at some 60 blocks an SM, and
+  // between 30 and that the rule loses up to a sixth.
   const int64_t work = (int64_t)p.blocks * p.tiles * ((a.M + 63) / 64);
   if (a.x_dtype == M3_BF16 && ((a.M > 32 && work >= 30ll * sm_count_current()) ||
                                (a.M > 16 && a.group == 128 && work >= 150ll * sm_count_current()))) {

@@ -177,10 +177,11 @@ struct TcPos {
   }
 };
 
-// cs: CTAs that split K; items: (128 weight rows, 128 batch rows) pairs
+// cs: CTAs that split K; items: (128 weight rows, NB batch rows) pairs
 template <int NB, int GPT>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    w4_tc_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tcodes, const W4Params p, int cs, int items) {
+    w4_tc_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tcodes, const W4Params p,
+                 int cs, int items) {
   using L = TcSmem<NB, GPT>;
   constexpr int READERS = NB == 64 && GPT == 1 ? 8 : 16, SETS = (kTcCopyCodes - READERS) / 4;
   extern __shared__ unsigned char tc_raw[];
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
   } else if (warp < kTcCopyCodes) {
-    // unpack: this warp's rows of every other tile, and their scales
+    // unpack: this warp's rows of every SETS-th tile, and their scales
     const int quarter = warp & 3, set = (warp - READERS) >> 2, lrow = quarter * 32 + lane;
     const int per = k1 - k0, total = item0 < items ? (items - item0 + istep - 1) / istep * per : 0;
     uint32_t zraw[GPT], sraw[GPT];  // zeros and scales of this warp's next tile, as they lie in memory

@@ -194,8 +194,11 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
 
     x is fp32 or bf16 with any row stride; the output has ``out_dtype`` (x's
     type by default).  Written for the batches of a decode step, right for
-    any M; from about 256 rows on the product with a bf16 weight is faster.  The codes' products with x must stay within fp32's range before
-    the scale; codes, scales and zeros take less than 4 GB each.  Inference
+    any M.  Of a bf16 x, up to 16 rows are faster than with an unquantised
+    weight, 32 about as fast or faster; beyond that the library's product
+    with a bf16 weight is faster, except for the largest weights (50,280 x
+    2,560: from 256 rows on).  The codes' products with x must stay within
+    fp32's range before the scale; codes, scales and zeros take less than 4 GB each.  Inference
     only: x or scales that ask for a gradient, also a forward-mode one, are
     refused."""
     global _host
