@@ -170,7 +170,7 @@ class Mamba3Decoder:
             if not self.use_triton_full_fused:
                 raise ValueError("w4_group_size needs use_triton_full_fused=True")
             self.use_single_launch = False  # that kernel streams unquantised weights
-            self._w4 = {name: W4Projection(lambda lin=getattr(model, name): lin.weight, w4_group_size)
+            self._w4 = {name: W4Projection(lambda name=name: getattr(model, name).weight, w4_group_size)
                         for name in ("in_proj", "out_proj")}
 
     # ------------------------------------------------------------------

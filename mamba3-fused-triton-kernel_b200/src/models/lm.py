@@ -39,6 +39,11 @@ from src.kernels.norm import residual_rmsnorm
 from src.models.inference import Mamba3Decoder, check_device_error
 
 
+def _linear(model, name: str, i: int):
+    """The model's LM head, or ``fc1`` / ``fc2`` of block ``i``'s MLP."""
+    return model.lm_head if name == "lm_head" else getattr(model.mlp_layers[i], name)
+
+
 class Mamba3LMDecoder:
     """Decoder over a ``MambaLMHeadModel``.  ``decoder_kwargs``: the
     ``Mamba3Decoder`` backend flags, applied to every layer;
@@ -61,12 +66,13 @@ class Mamba3LMDecoder:
         self._graph_states = None
         self._w4 = None
         if w4_group_size is not None:
-            linears = [model.lm_head] + [lin for mlp in model.mlp_layers or [] for lin in (mlp.fc1, mlp.fc2)]
-            self._w4 = {lin: W4Projection(lambda lin=lin: lin.weight, w4_group_size) for lin in linears}
+            places = [("lm_head", 0)] + [(fc, i) for i in range(len(model.mlp_layers or [])) for fc in ("fc1", "fc2")]
+            self._w4 = {at: W4Projection(lambda at=at: _linear(model, *at).weight, w4_group_size) for at in places}
 
-    def _weight(self, lin):
-        """The weight of an MLP layer or the LM head, or its 4-bit form."""
-        return lin.weight if self._w4 is None else self._w4[lin].get()
+    def _weight(self, name: str, i: int = 0):
+        """The weight of the LM head or of block ``i``'s MLP, or its 4-bit
+        form."""
+        return _linear(self.model, name, i).weight if self._w4 is None else self._w4[name, i].get()
 
     @property
     def vocab_size(self) -> int:
@@ -99,11 +105,11 @@ class Mamba3LMDecoder:
             o, _ = layer._graph_step_fn()(xn, st)
             if mlp is not None:
                 x, xm = residual_rmsnorm(x, o, m.mlp_norms[i].weight, m.mlp_norms[i].eps)
-                gate, val = linear(xm, self._weight(mlp[i].fc1)).chunk(2, dim=-1)
-                o = linear((F.silu(gate) * val).contiguous(), self._weight(mlp[i].fc2))
+                gate, val = linear(xm, self._weight("fc1", i)).chunk(2, dim=-1)
+                o = linear((F.silu(gate) * val).contiguous(), self._weight("fc2", i))
             nrm = self._norm_after(i)
             x, xn = residual_rmsnorm(x, o, nrm.weight, nrm.eps)
-        return linear(xn, self._weight(m.lm_head))
+        return linear(xn, self._weight("lm_head"))
 
     def warmup_cuda_graph(self, states: list, n_warmup: int = 3) -> None:
         """``n_warmup`` eager token steps (token id 0), then capture one token
