@@ -156,8 +156,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             the logits' type without it.
 
     Penalties given as tensors are not looked at by the host: a repetition
-    penalty is above 0.  Inference only: logits, a bias or penalties that ask
-    for a gradient, also a forward-mode one, are refused."""
+    penalty is above 0.  Inference only: logits, a bias, penalties or an out
+    that ask for a gradient, also a forward-mode one, are refused."""
     global _host_process
     if out is None:
         if _host_process is None:
@@ -177,6 +177,7 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             f"out must be a float32 or bfloat16 {(B, V)} tensor on the logits' device"
         assert (V <= 1 or out.stride(1) == 1) and (B <= 1 or out.stride(0) >= V), \
             "out must have unit column stride and rows that do not overlap"
+        _refuse_gradients(out)
         if out is not logits and _overlap(out, logits):
             assert out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and \
                 out.stride() == logits.stride(), "out may be the logits themselves, not overlap them otherwise"

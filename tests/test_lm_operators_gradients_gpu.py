@@ -59,3 +59,15 @@ def test_refused(name, i, python_path, monkeypatch):
                 call(*put(dual))
         assert torch.equal(call(*inputs), want)
     assert torch.equal(call(*inputs), want)
+
+
+def test_out_is_refused():
+    z = torch.randn(2, 100, device="cuda")
+    out = torch.full((2, 100), 7.0, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        process_logits(z, out=out)
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+        process_logits(z, out=fwAD.make_dual(out.detach(), torch.ones_like(z)))
+    assert bool((out == 7).all())
+    with torch.no_grad():
+        assert process_logits(z, out=out) is out and torch.equal(out, z)
