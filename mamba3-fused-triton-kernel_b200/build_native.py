@@ -123,8 +123,8 @@ def build_host(nvcc: str, force: bool = False) -> bool:
     libs = os.path.join(base, "lib")
     tmp = HOST_LIB + ".tmp"
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f'-DM3_TORCH_VERSION="{version}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + i for i in inc), HOST_SRC,
-           "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           f'-DM3_TORCH_VERSION="{version}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *("-I" + i for i in inc), HOST_SRC, "-o", tmp, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{r.stdout}\n{r.stderr}")

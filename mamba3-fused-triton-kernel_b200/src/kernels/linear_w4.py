@@ -198,9 +198,9 @@ def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
     weight, 32 about as fast or faster; beyond that the library's product
     with a bf16 weight is faster, except for the largest weights (50,280 x
     2,560: from 256 rows on).  The codes' products with x must stay within
-    fp32's range before the scale; codes, scales and zeros take less than 4 GB each.  Inference
-    only: x or scales that ask for a gradient, also a forward-mode one, are
-    refused."""
+    fp32's range before the scale; codes, scales and zeros take less than 4 GB
+    each.  Inference only: x or scales that ask for a gradient, also a
+    forward-mode one, are refused."""
     global _host
     if out_dtype is None:
         if _host is None:
