@@ -201,7 +201,7 @@ class Mamba3Decoder:
             step_fn(self._graph_input, state)
         torch.cuda.synchronize(device)
         self.check_device_error()
-        self._update_w4()
+        self.update_w4()
         self._cuda_graph = torch.cuda.CUDAGraph()
         self._host_graph = None
         self._host_output = None
@@ -302,6 +302,8 @@ class Mamba3Decoder:
         if state is None:
             state = self.init_state(batch, device=token_embeddings.device)
         outs = []
+        if self._cuda_graph is not None:
+            self.update_w4()
         for t in range(seq_len):
             out, state = self.step(token_embeddings[:, t], state)
             # graph replay returns one static buffer; keep each step's value
@@ -363,10 +365,15 @@ class Mamba3Decoder:
         model's, or its 4-bit form."""
         return getattr(self.model, name).weight if self._w4 is None else self._w4[name].get()
 
-    def _update_w4(self) -> None:
-        """Quantise what has changed now: it cannot be done in a capture."""
+    def update_w4(self, force: bool = False) -> None:
+        """Quantise the projections that have changed, in place (``force``:
+        all, for changes that PyTorch does not count).  An eager
+        step and ``prefill`` look for themselves; a captured step replays what
+        the 4-bit tensors hold, so it sees a changed weight after this (called
+        by ``warmup_cuda_graph`` and ``decode_sequence``).  Nothing to do
+        without ``w4_group_size``."""
         for projection in (self._w4 or {}).values():
-            projection.get()
+            projection.refresh() if force else projection.get()
 
     def _single_launch(self, state: dict, graph: bool = False):
         """Prepared single-launch step for this state and the current

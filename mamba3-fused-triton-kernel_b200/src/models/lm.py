@@ -122,14 +122,21 @@ class Mamba3LMDecoder:
             self._step_eager(self._graph_ids, states)
         torch.cuda.synchronize(h.device)
         self.check_device_error()
-        for layer in self.layers:
-            layer._update_w4()
-        for projection in (self._w4 or {}).values():
-            projection.get()
+        self.update_w4()
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):
             self._graph_logits = self._step_eager(self._graph_ids, states)
+
+    def update_w4(self, force: bool = False) -> None:
+        """Quantise the projections that have changed, in place: a captured
+        step sees a changed weight after this (``Mamba3Decoder.update_w4``).
+        Called by ``warmup_cuda_graph``, ``decode_sequence`` and
+        ``generate``."""
+        for layer in self.layers:
+            layer.update_w4(force)
+        for projection in (self._w4 or {}).values():
+            projection.refresh() if force else projection.get()
 
     def check_device_error(self) -> None:
         """Raise if a library kernel gave up a bounded wait since the last
@@ -158,6 +165,8 @@ class Mamba3LMDecoder:
         if states is None:
             states = self.init_state(B, device=input_ids.device)
         outs = []
+        if self._graph is not None:
+            self.update_w4()
         with torch.no_grad():
             for t in range(L):
                 logits, states = self.step(input_ids[:, t], states)
@@ -230,6 +239,8 @@ class Mamba3LMDecoder:
                         v.zero_()
             else:
                 states = self.init_state(B, device=dev)
+        if self._graph is not None:
+            self.update_w4()
         end = prompt + max_new_tokens
         lengths = prompt.clone()
         going = torch.ones(B, dtype=torch.bool, device=dev)

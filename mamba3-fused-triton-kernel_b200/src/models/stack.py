@@ -78,12 +78,18 @@ class Mamba3StackDecoder:
             self._step_eager(self._graph_input, states)
         torch.cuda.synchronize(h.device)
         check_device_error(self.layers)
-        for layer in self.layers:
-            layer._update_w4()
+        self.update_w4()
         self._graph = torch.cuda.CUDAGraph()
         self._graph_states = states
         with torch.cuda.graph(self._graph):
             self._graph_output, _ = self._step_eager(self._graph_input, states)
+
+    def update_w4(self, force: bool = False) -> None:
+        """Quantise the projections that have changed, in place: a captured
+        step sees a changed weight after this (``Mamba3Decoder.update_w4``).
+        Called by ``warmup_cuda_graph``."""
+        for layer in self.layers:
+            layer.update_w4(force)
 
     def step(self, x: torch.Tensor, states: list) -> tuple:
         """One token through every block: x (batch, d_model) -> (x_out, states)."""
